@@ -50,6 +50,9 @@ setup(
             name="avgen_b200._C",
             sources=sources(),
             include_dirs=[os.path.join(HERE, CSRC)],
+            # the shared C++ runtime torch uses: a toolchain that links its own static copy gives the
+            # extension a second set of locale facets, and an error message that formats a number crashes
+            extra_link_args=["-l:libstdc++.so.6"],
             extra_compile_args={"cxx": ["-O3", "-std=c++17"], "nvcc": NVCC_FLAGS},
         )
     ],
