@@ -9,6 +9,7 @@
 
 #include "include/host_utils.h"
 #include "include/launchers.h"
+#include "include/microscale.cuh"
 
 namespace avgen {
 bool install_crash_backtrace();  // crash_trace.cpp
@@ -898,6 +899,192 @@ void p2p_copy_py(int64_t dst, int64_t src, int64_t bytes) {
   p2p_copy(reinterpret_cast<void*>(dst), reinterpret_cast<const void*>(src), static_cast<size_t>(bytes), cur_stream());
 }
 
+// --------------------------------------------------------------------- block-scaled formats
+int mx_dtype(at::ScalarType t, const char* what) {
+  if (t == at::kBFloat16) return kMxBf16;
+  if (t == at::kHalf) return kMxFp16;
+  TORCH_CHECK(t == at::kFloat, what, " must be bf16, fp16 or fp32, got ", t);
+  return kMxFp32;
+}
+const float* mx_global(const OptT& g, const at::Tensor& like, const char* name) {
+  if (!has(g)) return nullptr;
+  check_f32(*g, name);
+  TORCH_CHECK(g->numel() == 1 && g->device() == like.device(), name, " must hold one fp32 value on the operand's device");
+  return g->data_ptr<float>();
+}
+// Codes and scales of a packed tensor of `cols` columns; returns its rows.
+long check_packed(const at::Tensor& codes, const at::Tensor& scales, int fmt, long cols, const char* name) {
+  TORCH_CHECK(fmt >= kMxFp8 && fmt <= kNvFp4, name, ": unknown format ", fmt);
+  TORCH_CHECK(cols > 0, name, ": needs at least one column");
+  check_cuda(codes, name);
+  TORCH_CHECK(codes.scalar_type() == at::kByte && codes.dim() == 2 && codes.is_contiguous() &&
+                  codes.size(1) == mx_row_bytes(fmt, cols),
+              name, ": codes must be contiguous uint8 [rows, ", mx_row_bytes(fmt, cols), "]");
+  TORCH_CHECK(scales.device() == codes.device() && scales.scalar_type() == at::kByte && scales.is_contiguous() &&
+                  scales.numel() == mx_scale_bytes(fmt, codes.size(0), cols),
+              name, ": scales must be contiguous uint8 of ", mx_scale_bytes(fmt, codes.size(0), cols),
+              " bytes on the codes' device");
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(codes.data_ptr()) % 16 == 0 &&
+                  reinterpret_cast<uintptr_t>(scales.data_ptr()) % 16 == 0,
+              name, ": codes and scales must be 16-byte aligned");
+  return codes.size(0);
+}
+at::Tensor mx_rows(const at::Tensor& x, const char* name) {
+  TORCH_CHECK(x.dim() >= 1 && x.size(-1) > 0, name, " needs a last dimension of at least one column");
+  const long cols = x.size(-1);
+  at::Tensor r = x.dim() == 2 ? x : x.reshape({x.numel() / cols, cols});
+  return cols > 1 && r.stride(1) != 1 ? r.contiguous() : r;
+}
+
+std::tuple<at::Tensor, at::Tensor, OptT> mx_quantize(const at::Tensor& x, int64_t fmt, const OptT& g, bool measure) {
+  check_cuda(x, "quantize: x");
+  c10::cuda::CUDAGuard guard(x.device());
+  const at::Tensor rows = mx_rows(x, "quantize: x");
+  TORCH_CHECK(fmt >= kMxFp8 && fmt <= kNvFp4, "quantize: unknown format ", fmt);
+  MxQuantDesc d;
+  d.device = x.device().index();
+  d.fmt = static_cast<int>(fmt);
+  d.dtype = mx_dtype(x.scalar_type(), "quantize: x");
+  d.rows = rows.size(0);
+  d.cols = rows.size(1);
+  d.x = rows.data_ptr();
+  d.ldx = rows.stride(0);
+  const auto bytes = x.options().dtype(at::kByte);
+  at::Tensor codes = at::empty({d.rows, mx_row_bytes(d.fmt, d.cols)}, bytes);
+  at::Tensor scales = at::empty({mx_scale_bytes(d.fmt, d.rows, d.cols)}, bytes);
+  d.codes = codes.data_ptr<uint8_t>();
+  d.scales = scales.data_ptr<uint8_t>();
+  d.g = mx_global(g, x, "quantize: global_scale");
+  OptT g_out = g;
+  if (fmt == kNvFp4 && measure) {
+    at::Tensor buf = at::empty({2}, x.options().dtype(at::kFloat));
+    if (d.rows == 0) buf.fill_(1.f);
+    g_out = buf.narrow(0, 0, 1);
+    d.g_out = buf.data_ptr<float>();
+    d.amax = reinterpret_cast<unsigned*>(buf.data_ptr<float>() + 1);
+  }
+  if (d.rows > 0) mx_quantize_launch(d, cur_stream());
+  return {codes, scales, g_out};
+}
+
+at::Tensor mx_dequantize(const at::Tensor& codes, const at::Tensor& scales, int64_t fmt, int64_t cols, const OptT& g,
+                         at::ScalarType dtype) {
+  MxDequantDesc d;
+  d.fmt = static_cast<int>(fmt);
+  d.rows = check_packed(codes, scales, d.fmt, cols, "dequantize");
+  c10::cuda::CUDAGuard guard(codes.device());
+  d.device = codes.device().index();
+  d.dtype = mx_dtype(dtype, "dequantize: dtype");
+  d.cols = cols;
+  d.codes = codes.data_ptr<uint8_t>();
+  d.scales = scales.data_ptr<uint8_t>();
+  d.g = mx_global(g, codes, "dequantize: global_scale");
+  at::Tensor out = at::empty({d.rows, cols}, codes.options().dtype(dtype));
+  d.out = out.data_ptr();
+  if (d.rows > 0) mx_dequantize_launch(d, cur_stream());
+  return out;
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> mx_add_rmsnorm(const at::Tensor& x, const OptT& update, const OptT& w,
+                                                              const OptT& scale, const OptT& shift, const OptT& gate,
+                                                              const OptT& groups, int64_t rows_per_batch, double eps,
+                                                              int64_t fmt, const OptT& g) {
+  check_cuda(x, "add_rmsnorm: x");
+  c10::cuda::CUDAGuard guard(x.device());
+  const at::Tensor rows = mx_rows(x, "add_rmsnorm: x");
+  TORCH_CHECK(fmt >= kMxFp8 && fmt <= kNvFp4, "add_rmsnorm: unknown format ", fmt);
+  MxNormDesc d;
+  d.device = x.device().index();
+  d.fmt = static_cast<int>(fmt);
+  d.dtype = mx_dtype(x.scalar_type(), "add_rmsnorm: x");
+  d.rows = rows.size(0);
+  TORCH_CHECK(rows.size(1) <= (1 << 20), "add_rmsnorm: at most ", 1 << 20, " columns, got ", rows.size(1));
+  d.W = static_cast<int>(rows.size(1));
+  d.eps = static_cast<float>(eps);
+  d.x = rows.data_ptr();
+  d.ldx = rows.stride(0);
+  at::Tensor u, out = x;
+  if (has(update)) {
+    TORCH_CHECK(update->sizes() == x.sizes() && update->scalar_type() == x.scalar_type() && update->device() == x.device(),
+                "add_rmsnorm: update must have x's shape, type and device");
+    u = mx_rows(*update, "add_rmsnorm: update");
+    d.update = u.data_ptr();
+    d.ldu = u.stride(0);
+    out = at::empty(x.sizes(), x.options());
+    d.x_out = out.data_ptr();
+  }
+  d.rows_per_batch = std::max<int64_t>(1, rows_per_batch);
+  d.g = mx_global(g, x, "add_rmsnorm: global_scale");
+  d.w = f32_or_null(w, "add_rmsnorm: weight");
+  TORCH_CHECK(d.w == nullptr || (w->numel() == d.W && w->device() == x.device()), "add_rmsnorm: weight must be fp32 [",
+              d.W, "] on x's device");
+  TORCH_CHECK(!has(gate) || has(update), "add_rmsnorm: gate needs an update");
+  long mod_rows = -1;
+  auto mod = [&](const OptT& t, const char* name) -> const float* {
+    if (!has(t)) return nullptr;
+    check_f32(*t, name);
+    TORCH_CHECK(t->dim() == 2 && t->size(0) > 0 && t->size(1) == d.W && (d.W == 1 || t->stride(1) == 1) && t->device() == x.device(),
+                "add_rmsnorm: ", name, " must be fp32 [rows, ", d.W, "] with contiguous rows on x's device");
+    TORCH_CHECK(mod_rows < 0 || t->size(0) == mod_rows, "add_rmsnorm: scale, shift and gate differ in their rows");
+    mod_rows = t->size(0);
+    return t->data_ptr<float>();
+  };
+  d.scale = mod(scale, "scale");
+  d.shift = mod(shift, "shift");
+  d.gate = mod(gate, "gate");
+  if (d.scale != nullptr) d.mod_stride = scale->stride(0);
+  if (d.shift != nullptr) {
+    TORCH_CHECK(d.scale == nullptr || shift->stride(0) == d.mod_stride, "add_rmsnorm: scale and shift strides differ");
+    d.mod_stride = shift->stride(0);
+  }
+  if (d.gate != nullptr) d.gate_stride = gate->stride(0);
+  if (mod_rows >= 0) {
+    d.groups = groups_or_null(groups, d.rows, "add_rmsnorm");
+    TORCH_CHECK(d.groups == nullptr || groups->device() == x.device(), "add_rmsnorm: groups must be on x's device");
+    d.num_groups = static_cast<int>(mod_rows);
+    TORCH_CHECK(d.groups != nullptr || mod_rows * d.rows_per_batch >= d.rows,
+                "add_rmsnorm: modulation rows do not cover x");
+  }
+  const auto bytes = x.options().dtype(at::kByte);
+  at::Tensor codes = at::empty({d.rows, mx_row_bytes(d.fmt, d.W)}, bytes);
+  at::Tensor scales = at::empty({mx_scale_bytes(d.fmt, d.rows, d.W)}, bytes);
+  d.codes = codes.data_ptr<uint8_t>();
+  d.scales = scales.data_ptr<uint8_t>();
+  if (d.rows > 0) mx_add_rmsnorm_launch(d, cur_stream());
+  return {out, codes, scales};
+}
+
+at::Tensor mx_gemm(const at::Tensor& a_codes, const at::Tensor& a_scales, const OptT& a_g, const at::Tensor& b_codes,
+                   const at::Tensor& b_scales, const OptT& b_g, int64_t fmt, int64_t k, const OptT& bias,
+                   at::ScalarType dtype) {
+  MxGemmDesc d;
+  d.fmt = static_cast<int>(fmt);
+  const long m = check_packed(a_codes, a_scales, d.fmt, k, "matmul: a");
+  const long n = check_packed(b_codes, b_scales, d.fmt, k, "matmul: b");
+  TORCH_CHECK(a_codes.device() == b_codes.device(), "matmul: operands on different devices");
+  TORCH_CHECK(m < (1L << 31) - 256 && n < (1L << 31) - 256 && k < (1L << 30), "matmul: sizes beyond 32 bits");
+  c10::cuda::CUDAGuard guard(a_codes.device());
+  d.device = a_codes.device().index();
+  d.dtype = mx_dtype(dtype, "matmul: out_dtype");
+  d.M = static_cast<int>(m);
+  d.N = static_cast<int>(n);
+  d.K = static_cast<int>(k);
+  d.a_codes = a_codes.data_ptr<uint8_t>();
+  d.a_scales = a_scales.data_ptr<uint8_t>();
+  d.b_codes = b_codes.data_ptr<uint8_t>();
+  d.b_scales = b_scales.data_ptr<uint8_t>();
+  d.a_g = mx_global(a_g, a_codes, "matmul: a's global_scale");
+  d.b_g = mx_global(b_g, b_codes, "matmul: b's global_scale");
+  d.bias = f32_or_null(bias, "matmul: bias");
+  TORCH_CHECK(d.bias == nullptr || (bias->numel() == n && bias->device() == a_codes.device()),
+              "matmul: bias must be fp32 [", n, "] on the operands' device");
+  at::Tensor out = at::empty({m, n}, a_codes.options().dtype(dtype));
+  d.out = out.data_ptr();
+  d.err = error_word(d.device);
+  if (m > 0 && n > 0) mx_gemm_launch(d, cur_stream());
+  return out;
+}
+
 int64_t read_error(int64_t device) {
   int v = 0;
   AVGEN_CUDA_CHECK(cudaMemcpy(&v, error_word(static_cast<int>(device)), sizeof(int), cudaMemcpyDeviceToHost));
@@ -979,6 +1166,13 @@ PYBIND11_MODULE(_C, m) {
   m.def("slab_sum", &a::slab_sum, arg("srcs"), arg("dst"));
   m.def("install_crash_backtrace", &avgen::install_crash_backtrace,
         "print native frames on SIGSEGV/SIGBUS/SIGFPE/SIGILL/SIGABRT, then chain to the previous handler");
+  m.def("mx_quantize", &a::mx_quantize, arg("x"), arg("fmt"), arg("global_scale") = none, arg("measure") = false);
+  m.def("mx_dequantize", &a::mx_dequantize, arg("codes"), arg("scales"), arg("fmt"), arg("cols"), arg("global_scale"),
+        arg("dtype"));
+  m.def("mx_add_rmsnorm", &a::mx_add_rmsnorm, arg("x"), arg("update"), arg("weight"), arg("scale"), arg("shift"),
+        arg("gate"), arg("groups"), arg("rows_per_batch"), arg("eps"), arg("fmt"), arg("global_scale"));
+  m.def("mx_gemm", &a::mx_gemm, arg("a_codes"), arg("a_scales"), arg("a_global"), arg("b_codes"), arg("b_scales"),
+        arg("b_global"), arg("fmt"), arg("k"), arg("bias"), arg("dtype"));
   m.def("read_error", &a::read_error);
   m.def("clear_error", &a::clear_error);
 }

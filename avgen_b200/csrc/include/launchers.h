@@ -379,4 +379,82 @@ void mt_sq_norm_launch(const MTChunk* chunks, int nchunks, const MTTensor* tenso
 void mt_adamw_launch(const MTChunk* chunks, int nchunks, const MTTensor* tensors, const MTAdamWArgs& args,
                      cudaStream_t stream);
 
+// Block-scaled formats (microscale.cu, mx_gemm.cu; the formats themselves are in
+// microscale.cuh). `fmt` is an MxFormat; `dtype` is the type of the plain tensor.
+enum MxDType : int { kMxBf16 = 0, kMxFp16 = 1, kMxFp32 = 2 };
+
+struct MxQuantDesc {
+  int device = 0;
+  int fmt = 0;
+  int dtype = 0;
+  long rows = 0, cols = 0;
+  const void* x = nullptr;  // [rows, cols], row stride ldx elements
+  long ldx = 0;
+  uint8_t* codes = nullptr;   // [rows, mx_row_bytes]
+  uint8_t* scales = nullptr;  // [mx_scale_bytes]
+  const float* g = nullptr;   // nvfp4: the caller's tensor scale, or
+  unsigned* amax = nullptr;   // scratch word from which one is made, stored in
+  float* g_out = nullptr;
+};
+void mx_quantize_launch(const MxQuantDesc& d, cudaStream_t stream);
+
+struct MxDequantDesc {
+  int device = 0;
+  int fmt = 0;
+  int dtype = 0;
+  long rows = 0, cols = 0;
+  const uint8_t* codes = nullptr;
+  const uint8_t* scales = nullptr;
+  const float* g = nullptr;
+  void* out = nullptr;  // [rows, cols] contiguous
+};
+void mx_dequantize_launch(const MxDequantDesc& d, cudaStream_t stream);
+
+// x_out = x + gate[b] * update; the norm of that sum, modulated as rmsnorm_mod does,
+// quantised. update may be null (x_out is then null too).
+struct MxNormDesc {
+  int device = 0;
+  int fmt = 0;
+  int dtype = 0;
+  long rows = 0;
+  int W = 0;
+  float eps = 1e-6f;
+  const void* x = nullptr;
+  long ldx = 0;
+  const void* update = nullptr;
+  long ldu = 0;
+  void* x_out = nullptr;  // [rows, W] contiguous
+  const float* w = nullptr;
+  const float* scale = nullptr;
+  const float* shift = nullptr;
+  long mod_stride = 0;
+  const float* gate = nullptr;
+  long gate_stride = 0;
+  const int* groups = nullptr;
+  int num_groups = 0;
+  long rows_per_batch = 1;
+  uint8_t* codes = nullptr;
+  uint8_t* scales = nullptr;
+  const float* g = nullptr;
+};
+void mx_add_rmsnorm_launch(const MxNormDesc& d, cudaStream_t stream);
+
+// out[M, N] = A[M, K] . B[N, K]^T (+ bias), both operands in format `fmt`.
+struct MxGemmDesc {
+  int device = 0;
+  int fmt = 0;
+  int dtype = 0;  // of out
+  int M = 0, N = 0, K = 0;
+  const uint8_t* a_codes = nullptr;
+  const uint8_t* a_scales = nullptr;
+  const float* a_g = nullptr;
+  const uint8_t* b_codes = nullptr;
+  const uint8_t* b_scales = nullptr;
+  const float* b_g = nullptr;
+  const float* bias = nullptr;  // [N]
+  void* out = nullptr;          // [M, N] contiguous
+  int* err = nullptr;
+};
+void mx_gemm_launch(const MxGemmDesc& d, cudaStream_t stream);
+
 }  // namespace avgen
