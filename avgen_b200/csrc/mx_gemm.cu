@@ -6,12 +6,19 @@
 // accumulate in fp32 (kind::mxf8f6f4 / mxf4 / mxf4nvf4 with .block_scale), so the
 // operands stay packed all the way; alpha = g_a * g_b is nvfp4's pair of tensor scales.
 //
-// Structure (one CTA per SM, persistent over output tiles):
-//   warp 0      producer: per k-block (128 code bytes of each row) the A and B tiles
-//               by TMA, their scale tiles by bulk copies, into a ring
-//   warp 1      MMA issuer: copies a stage's scales to TMEM (tcgen05.cp), then issues
-//               its products; the two kinds of instruction execute in issue order
-//   warps 2..5  epilogue, one TMEM lane quadrant each
+// Structure (persistent over output tiles; CTAS = 2 pairs the two SMs of a TPC on one
+// 256 x 256 tile, CTAS = 1 gives each SM a 128 x 128 tile):
+//   warp 0      producer: per k-block (128 code bytes of each row) this CTA's A and B
+//               rows and the scale tiles by TMA into a ring
+//   warp 1      MMA issuer (the pair's first CTA): copies a stage's scales to TMEM
+//               (tcgen05.cp), then issues its products; both kinds of instruction
+//               execute in issue order
+//   warps 2..5  epilogue, one TMEM lane quadrant (32 rows) each: TMEM -> registers ->
+//               shared memory -> TMA store, 128 bytes of each row at a time
+//
+// In a pair each CTA stages its own 128 rows of A and half of B's 256 rows: the same
+// operand bytes from L2 and shared memory per product as one SM would need for half
+// the work.
 #include <algorithm>
 
 #include "include/host_utils.h"
@@ -23,11 +30,9 @@ namespace avgen {
 namespace {
 
 struct MxArgs {
-  int M, N, K;
-  int row_bytes;  // of a row's codes
-  int tiles_k;    // scale tiles along K
-  const uint8_t* a_scales;
-  const uint8_t* b_scales;
+  int M, N;
+  int num_kb;      // k-blocks
+  int last_steps;  // products in the last one
   const float* a_g;
   const float* b_g;
   const float* bias;
@@ -35,81 +40,253 @@ struct MxArgs {
   int* err;
 };
 
-constexpr int kBM = 128;
+constexpr int kBM = 128;        // rows of A per CTA
 constexpr int kRowBytes = 128;  // code bytes of a row in one k-block: one swizzle row
 constexpr int kSteps = 4;       // products per k-block, 32 code bytes each
+constexpr int kBoxBytes = 32 * 128;  // one warp's store: 32 rows x 128 bytes
+constexpr int kSmemLimit = 232448;
 
-template <int FMT, int BN>
+template <int FMT, int BN, int CTAS>
 struct Cfg {
   static constexpr int SF_TILES = FMT == kNvFp4 ? 4 : FMT == kMxFp4 ? 2 : 1;  // scale tiles per k-block
+  static constexpr int B_ROWS = BN / CTAS;
   static constexpr int A_BYTES = kBM * kRowBytes;
-  static constexpr int B_BYTES = BN * kRowBytes;
+  static constexpr int B_BYTES = B_ROWS * kRowBytes;
   static constexpr int SFA_BYTES = SF_TILES * 512;
-  static constexpr int SFB_BYTES = BN / 128 * SF_TILES * 512;
-  static constexpr int STAGE_BYTES = (A_BYTES + B_BYTES + SFA_BYTES + SFB_BYTES + 1023) / 1024 * 1024;
-  static constexpr int STAGES = (232448 - 2048) / STAGE_BYTES;
-  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 256;
-  static constexpr int SF_COL = 2 * BN;  // TMEM columns of the scales, after both accumulators
-  static constexpr int SFB_COL = SF_COL + SF_TILES * 4;
-  static constexpr int TMEM_COLS = 512;
+  static constexpr int SFB_BYTES = BN / 128 * SF_TILES * 512;  // of all BN rows, in both CTAs
+  static constexpr int TX_BYTES = A_BYTES + B_BYTES + SFA_BYTES + SFB_BYTES;
+  static constexpr int STAGE_BYTES = (TX_BYTES + 1023) / 1024 * 1024;
+  static constexpr int OUT_BYTES = 4 * 2 * kBoxBytes;
+  static constexpr int STAGES = std::min(8, (kSmemLimit - 2048 - OUT_BYTES) / STAGE_BYTES);
+  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + OUT_BYTES + 1024 + 256;
+  // TMEM: two accumulators and the scales of one k-block. Two 256-column accumulators
+  // leave no room for scales, so the second starts inside the first: the epilogue reads
+  // the shared columns first and hands them over, and the next tile's products wait for
+  // that instead of for a free accumulator.
+  static constexpr int SF_COLS = (SF_TILES * 4 * (1 + BN / 128) + 31) / 32 * 32;
+  static constexpr bool OVERLAP = 2 * BN + SF_COLS > 512;
+  static constexpr int ACC1 = OVERLAP ? 512 - SF_COLS - BN : BN;
+  static constexpr int SF_COL = ACC1 + BN;
 };
 
 // Instruction descriptor of the block-scaled kinds: element types, scale type, shape.
-// The positions of the scales inside a 32-bit TMEM cell (4, 29) vary by step.
+// The positions of the scales inside a 32-bit TMEM cell (bits 4 and 29) vary by step.
 template <int FMT>
 constexpr uint32_t mx_idesc(int m, int n) {
-  const uint32_t type = FMT == kMxFp8 ? 0u : 1u;    // e4m3 / e2m1
-  const uint32_t scale = FMT == kNvFp4 ? 0u : 1u;   // e4m3 / e8m0
+  const uint32_t type = FMT == kMxFp8 ? 0u : 1u;   // e4m3 / e2m1
+  const uint32_t scale = FMT == kNvFp4 ? 0u : 1u;  // e4m3 / e8m0
   return (type << 7) | (type << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (scale << 23) |
          (static_cast<uint32_t>(m >> 7) << 27);
 }
 
-template <int FMT>
+template <int FMT, int CTAS>
 __device__ __forceinline__ void mx_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
                                        uint32_t accumulate) {
-#define AVGEN_MX_MMA(KIND)                                                                    \
-  asm volatile(                                                                               \
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"                                       \
-      "tcgen05.mma.cta_group::1." KIND " [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),     \
-      "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)                         \
+#define AVGEN_MX_MMA(CG, KIND)                                                            \
+  asm volatile(                                                                           \
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"                                   \
+      "tcgen05.mma.cta_group::" CG "." KIND " [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d), \
+      "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)                     \
       : "memory")
-  if constexpr (FMT == kMxFp8) AVGEN_MX_MMA("kind::mxf8f6f4.block_scale.scale_vec::1X");
-  if constexpr (FMT == kMxFp4) AVGEN_MX_MMA("kind::mxf4.block_scale.scale_vec::2X");
-  if constexpr (FMT == kNvFp4) AVGEN_MX_MMA("kind::mxf4nvf4.block_scale.scale_vec::4X");
+  if constexpr (CTAS == 1) {
+    if constexpr (FMT == kMxFp8) AVGEN_MX_MMA("1", "kind::mxf8f6f4.block_scale.scale_vec::1X");
+    if constexpr (FMT == kMxFp4) AVGEN_MX_MMA("1", "kind::mxf4.block_scale.scale_vec::2X");
+    if constexpr (FMT == kNvFp4) AVGEN_MX_MMA("1", "kind::mxf4nvf4.block_scale.scale_vec::4X");
+  } else {
+    if constexpr (FMT == kMxFp8) AVGEN_MX_MMA("2", "kind::mxf8f6f4.block_scale.scale_vec::1X");
+    if constexpr (FMT == kMxFp4) AVGEN_MX_MMA("2", "kind::mxf4.block_scale.scale_vec::2X");
+    if constexpr (FMT == kNvFp4) AVGEN_MX_MMA("2", "kind::mxf4nvf4.block_scale.scale_vec::4X");
+  }
 #undef AVGEN_MX_MMA
 }
 
 // One scale tile (512 bytes of shared memory: 32 rows of 16 bytes) to four TMEM
-// columns, repeated in all four lane quadrants.
+// columns, repeated in all four lane quadrants; in a pair, in each CTA from its own
+// shared memory.
+template <int CTAS>
 __device__ __forceinline__ void copy_scales(uint32_t taddr, uint32_t smem_addr) {
   const uint64_t desc = static_cast<uint64_t>((smem_addr >> 4) & 0x3FFFu) | (static_cast<uint64_t>(128 >> 4) << 32) |
                         (1ull << 46);  // no swizzle, 8-row groups 128 bytes apart
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+  if constexpr (CTAS == 1)
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+  else
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
 
-// Bytes of 16-byte granularity from global to shared memory.
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                   smem_u32(dst)),
-               "l"(src), "r"(bytes), "r"(smem_u32(bar))
-               : "memory");
-}
-
-__device__ __forceinline__ void drain_wait(uint64_t* bar, uint32_t parity) {
-  const uint32_t a = smem_u32(bar);
-  const uint64_t t0 = globaltimer();
-  while (!mbar_try_wait(a, parity)) {
-    if (globaltimer() - t0 > kWaitTimeoutNs) return;
+// The scales and products of one staged k-block.
+template <int FMT, int BN, int CTAS>
+__device__ __forceinline__ void issue_block(uint32_t stage_addr, uint32_t tmem_sf, uint32_t tmem_acc, uint32_t idesc,
+                                            int steps, bool first) {
+  using C = Cfg<FMT, BN, CTAS>;
+  constexpr int SFB_TILES = (BN + 127) / 128;
+  constexpr int PER = kSteps / C::SF_TILES;  // products per scale tile
+  const uint32_t sa = stage_addr, sb = sa + C::A_BYTES, sfa = sb + C::B_BYTES, sfb = sfa + C::SFA_BYTES;
+  const uint32_t t_sfb = tmem_sf + C::SF_TILES * 4;
+#pragma unroll
+  for (int i = 0; i < C::SF_TILES; ++i) {
+    copy_scales<CTAS>(tmem_sf + 4 * i, sfa + 512 * i);
+#pragma unroll
+    for (int j = 0; j < SFB_TILES; ++j)
+      copy_scales<CTAS>(t_sfb + (i * SFB_TILES + j) * 4, sfb + j * C::SFA_BYTES + 512 * i);
+  }
+#pragma unroll
+  for (int k = 0; k < kSteps; ++k) {
+    if (k < steps) {
+      const uint32_t id = static_cast<uint32_t>(k % PER * (4 / PER));  // the step's first scale in its 4-byte cell
+      mx_mma<FMT, CTAS>(tmem_acc, umma_desc_sw128(sa + 32 * k, 16, 1024), umma_desc_sw128(sb + 32 * k, 16, 1024),
+                        idesc | (id << 4) | (id << 29), tmem_sf + 4 * (k / PER), t_sfb + (k / PER) * SFB_TILES * 4,
+                        (!first || k > 0) ? 1u : 0u);
+    }
   }
 }
 
-template <typename T, int FMT, int BN>
+// ---------------------------------------------------------------- pair plumbing
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void arrive_at(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
+// TMA loads whose completion is counted at `bar`, a shared::cluster address (in a pair:
+// of the first CTA).
+template <int CTAS>
+__device__ __forceinline__ void load_2d(void* dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
+  if constexpr (CTAS == 1)
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
+            smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, "
+        "%4}], [%2];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
+        : "memory");
+}
+template <int CTAS>
+__device__ __forceinline__ void load_3d(void* dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
+  if constexpr (CTAS == 1)
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::
+            "r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, "
+        "%5}], [%2];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+__device__ __forceinline__ void store_2d(const CUtensorMap* map, const void* src, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(smem_u32(src)), "r"(x), "r"(y)
+               : "memory");
+}
+
+// Arrive at `bar` (in a pair: at this offset in both CTAs) when every tcgen05 operation
+// this thread issued so far is done.
+template <int CTAS>
+__device__ __forceinline__ void commit(uint64_t* bar) {
+  if constexpr (CTAS == 1)
+    mma_commit(bar);
+  else
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            smem_u32(bar)),
+        "h"(static_cast<uint16_t>(3))
+        : "memory");
+}
+template <int CTAS>
+__device__ __forceinline__ void alloc_tmem(uint32_t* slot) {
+  if constexpr (CTAS == 1) {
+    tmem_alloc(slot, 512);
+    tmem_relinquish();
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(slot)));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+  }
+}
+template <int CTAS>
+__device__ __forceinline__ void free_tmem(uint32_t taddr) {
+  if constexpr (CTAS == 1)
+    tmem_dealloc(taddr, 512);
+  else
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(taddr));
+}
+
+// After an abort: copies still in flight land well within a millisecond.
+__device__ __forceinline__ void let_copies_land() {
+  const uint64_t t0 = globaltimer();
+  while (globaltimer() - t0 < 1000000ull) __nanosleep(1000);
+}
+
+// Grouped raster: 8 row tiles share each sweep over the columns, so that the tiles in
+// flight together re-read few operand rows from L2.
+__device__ __forceinline__ void tile_at(int t, int num_m, int num_n, int& tm, int& tn) {
+  constexpr int G = 8;
+  const int group = t / (G * num_n);
+  const int rows = min(G, num_m - group * G);
+  const int r = t - group * G * num_n;
+  tm = group * G + r % rows;
+  tn = r / rows;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  return pack_bf16(lo, hi);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// Stages one row's 128 bytes (64 16-bit or 32 fp32 values) of a 32-row store box in
+// the 128-byte swizzle: 16-byte chunk j of row r at chunk j ^ (r % 8).
+template <typename T>
+__device__ __forceinline__ void stage_row(uint8_t* box, int lane, const float* v) {
+  uint4* row = reinterpret_cast<uint4*>(box + lane * 128);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    uint4 w;
+    if constexpr (sizeof(T) == 2) {
+      w = make_uint4(pack2<T>(v[8 * j], v[8 * j + 1]), pack2<T>(v[8 * j + 2], v[8 * j + 3]),
+                     pack2<T>(v[8 * j + 4], v[8 * j + 5]), pack2<T>(v[8 * j + 6], v[8 * j + 7]));
+    } else {
+      w = make_uint4(__float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]), __float_as_uint(v[4 * j + 2]),
+                     __float_as_uint(v[4 * j + 3]));
+    }
+    row[j ^ (lane & 7)] = w;
+  }
+}
+
+template <typename T, int FMT, int BN, int CTAS>
 __global__ void __launch_bounds__(192, 1)
-    mx_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const MxArgs args) {
-  using C = Cfg<FMT, BN>;
+    mx_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                   const __grid_constant__ CUtensorMap tmSFA, const __grid_constant__ CUtensorMap tmSFB,
+                   const __grid_constant__ CUtensorMap tmOut, const bool tma_out, const MxArgs args) {
+  using C = Cfg<FMT, BN, CTAS>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::STAGES * C::STAGE_BYTES);
+  uint8_t* smem_out = smem + C::STAGES * C::STAGE_BYTES;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem_out + C::OUT_BYTES);
   uint64_t* empty = full + C::STAGES;
   uint64_t* tfull = empty + C::STAGES;
   uint64_t* tempty = tfull + 2;
@@ -118,11 +295,11 @@ __global__ void __launch_bounds__(192, 1)
 
   const int warp = warp_id();
   const int lane = lane_id();
-  const int num_m = (args.M + kBM - 1) / kBM;
+  const int rank = CTAS == 2 ? static_cast<int>(cluster_rank()) : 0;
+  const int num_m = (args.M + CTAS * kBM - 1) / (CTAS * kBM);
   const int num_n = (args.N + BN - 1) / BN;
   const int num_tiles = num_m * num_n;
-  const int num_kb = (args.row_bytes + kRowBytes - 1) / kRowBytes;
-  const int last_steps = (args.row_bytes - (num_kb - 1) * kRowBytes + 31) / 32;
+  const int first = blockIdx.x / CTAS, step = gridDim.x / CTAS;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::STAGES; ++s) {
@@ -131,29 +308,34 @@ __global__ void __launch_bounds__(192, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&tfull[b], 1);
-      mbar_init(&tempty[b], 128);
+      mbar_init(&tempty[b], 4 * CTAS);
     }
     *abort_flag = 0;
     fence_barrier_init();
   }
-  if (warp == 1) {
-    tmem_alloc(tmem_slot, C::TMEM_COLS);
-    tmem_relinquish();
+  if (warp == 0 && lane == 0) {
+    prefetch_tmap(&tmA);
+    prefetch_tmap(&tmB);
+    prefetch_tmap(&tmSFA);
+    prefetch_tmap(&tmSFB);
+    if (tma_out) prefetch_tmap(&tmOut);
   }
+  if (warp == 1) alloc_tmem<CTAS>(tmem_slot);
   tc_fence_before();
-  __syncthreads();
+  if constexpr (CTAS == 2) cluster_sync();
+  else __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
   if (warp == 0) {
     if (lane == 0) {
-      int stage = 0, issued = 0;
+      int stage = 0;
       uint32_t phase = 0;
       bool aborted = false;
-      for (int t = blockIdx.x; t < num_tiles && !aborted; t += gridDim.x) {
-        const int tm = t % num_m, tn = t / num_m;
-        const int b_groups = min(BN, args.N - tn * BN + 127) / 128;  // 128-row scale groups this tile has
-        for (int kb = 0; kb < num_kb; ++kb) {
+      for (int t = first; t < num_tiles && !aborted; t += step) {
+        int tm, tn;
+        tile_at(t, num_m, num_n, tm, tn);
+        for (int kb = 0; kb < args.num_kb; ++kb) {
           if (!mbar_wait(&empty[stage], phase ^ 1, abort_flag, args.err, kErrTimeoutProducer)) {
             aborted = true;
             break;
@@ -162,157 +344,216 @@ __global__ void __launch_bounds__(192, 1)
           uint8_t* sb = sa + C::A_BYTES;
           uint8_t* sfa = sb + C::B_BYTES;
           uint8_t* sfb = sfa + C::SFA_BYTES;
-          const int tile0 = kb * C::SF_TILES;
-          const uint32_t sf_bytes = static_cast<uint32_t>(min(C::SF_TILES, args.tiles_k - tile0)) * 512u;
-          mbar_arrive_expect_tx(&full[stage], C::A_BYTES + C::B_BYTES + sf_bytes * (1 + b_groups));
-          tma_load_2d(sa, &tmA, &full[stage], kb * kRowBytes, tm * kBM);
-          tma_load_2d(sb, &tmB, &full[stage], kb * kRowBytes, tn * BN);
-          bulk_load(sfa, args.a_scales + (static_cast<long>(tm) * args.tiles_k + tile0) * 512, sf_bytes, &full[stage]);
-          for (int j = 0; j < b_groups; ++j)
-            bulk_load(sfb + j * C::SFA_BYTES,
-                      args.b_scales + (static_cast<long>(tn * (BN / 128) + j) * args.tiles_k + tile0) * 512, sf_bytes,
-                      &full[stage]);
-          ++issued;
+          if (rank == 0) mbar_arrive_expect_tx(&full[stage], CTAS * C::TX_BYTES);
+          const uint32_t bar = CTAS == 2 ? map_to_rank(smem_u32(&full[stage]), 0) : smem_u32(&full[stage]);
+          load_2d<CTAS>(sa, &tmA, bar, kb * kRowBytes, (tm * CTAS + rank) * kBM);
+          load_2d<CTAS>(sb, &tmB, bar, kb * kRowBytes, tn * BN + rank * C::B_ROWS);
+          load_3d<CTAS>(sfa, &tmSFA, bar, 0, kb * C::SF_TILES, tm * CTAS + rank);
+          load_3d<CTAS>(sfb, &tmSFB, bar, 0, kb * C::SF_TILES, tn * (BN / 128));
           if (++stage == C::STAGES) {
             stage = 0;
             phase ^= 1;
           }
         }
       }
-      if (aborted) {  // copies in flight land before the CTA's shared memory goes away
-        for (int i = 0; i < min(issued, C::STAGES); ++i) {
-          if (--stage < 0) {
-            stage = C::STAGES - 1;
-            phase ^= 1;
-          }
-          drain_wait(&full[stage], phase);
-        }
-      }
+      if (aborted) let_copies_land();
     }
   } else if (warp == 1) {
-    constexpr uint32_t idesc = mx_idesc<FMT>(kBM, BN);
-    int stage = 0, acc = 0;
-    uint32_t phase = 0, acc_phase = 0;
-    bool aborted = false;
-    for (int t = blockIdx.x; t < num_tiles && !aborted; t += gridDim.x) {
-      if (!mbar_wait(&tempty[acc], acc_phase ^ 1, abort_flag, args.err, kErrTimeoutMma)) break;
-      tc_fence_after();
-      for (int kb = 0; kb < num_kb; ++kb) {
-        if (!mbar_wait(&full[stage], phase, abort_flag, args.err, kErrTimeoutMma)) {
-          aborted = true;
-          break;
-        }
+    if (rank == 0) {
+      constexpr uint32_t idesc = mx_idesc<FMT>(CTAS * kBM, BN);
+      int stage = 0;
+      uint32_t phase = 0;
+      bool aborted = false;
+      int i = 0;  // tiles done by this CTA
+      for (int t = first; t < num_tiles && !aborted; t += step, ++i) {
+        const int acc = i & 1;
+        // the tile that must have been read (its shared columns, or all of it) before this one
+        const int before = C::OVERLAP ? i - 1 : i - 2;
+        if (before >= 0 && !mbar_wait(&tempty[before & 1], (before >> 1) & 1, abort_flag, args.err, kErrTimeoutMma)) break;
         tc_fence_after();
-        if (elect_one()) {
-          const uint32_t sa = smem_u32(smem + stage * C::STAGE_BYTES);
-          const uint32_t sb = sa + C::A_BYTES;
-          const uint32_t sfa = sb + C::B_BYTES;
-          const uint32_t sfb = sfa + C::SFA_BYTES;
-#pragma unroll
-          for (int i = 0; i < C::SF_TILES; ++i) {
-            copy_scales(tmem + C::SF_COL + 4 * i, sfa + 512 * i);
-#pragma unroll
-            for (int j = 0; j < BN / 128; ++j)
-              copy_scales(tmem + C::SFB_COL + (i * (BN / 128) + j) * 4, sfb + j * C::SFA_BYTES + 512 * i);
+        for (int kb = 0; kb < args.num_kb; ++kb) {
+          if (!mbar_wait(&full[stage], phase, abort_flag, args.err, kErrTimeoutMma)) {
+            aborted = true;
+            break;
           }
-          const int steps = kb == num_kb - 1 ? last_steps : kSteps;
-#pragma unroll
-          for (int k = 0; k < kSteps; ++k) {
-            if (k < steps) {
-              constexpr int PER = kSteps / C::SF_TILES;                        // steps per scale tile
-              const uint32_t id = static_cast<uint32_t>(k % PER * (4 / PER));  // byte of the first scale
-              const int i = k / PER;
-              mx_mma<FMT>(tmem + acc * BN, umma_desc_sw128(sa + 32 * k, 16, 1024), umma_desc_sw128(sb + 32 * k, 16, 1024),
-                          idesc | (id << 4) | (id << 29), tmem + C::SF_COL + 4 * i,
-                          tmem + C::SFB_COL + i * (BN / 128) * 4, (kb > 0 || k > 0) ? 1u : 0u);
-            }
+          tc_fence_after();
+          if (elect_one()) {
+            issue_block<FMT, BN, CTAS>(smem_u32(smem + stage * C::STAGE_BYTES), tmem + C::SF_COL, tmem + acc * C::ACC1,
+                                       idesc, kb == args.num_kb - 1 ? args.last_steps : kSteps, kb == 0);
+            commit<CTAS>(&empty[stage]);
           }
-          mma_commit(&empty[stage]);
+          __syncwarp();
+          if (++stage == C::STAGES) {
+            stage = 0;
+            phase ^= 1;
+          }
         }
+        if (aborted) break;
+        if (elect_one()) commit<CTAS>(&tfull[acc]);
         __syncwarp();
-        if (++stage == C::STAGES) {
-          stage = 0;
-          phase ^= 1;
-        }
       }
-      if (aborted) break;
-      if (elect_one()) mma_commit(&tfull[acc]);
-      __syncwarp();
-      acc ^= 1;
-      if (acc == 0) acc_phase ^= 1;
     }
   } else {
+    constexpr int GROUPS = BN / 64;                  // of 64 columns
+    constexpr int BOX = 128 / static_cast<int>(sizeof(T));  // columns of a store box
     const int q = warp & 3;
-    int acc = 0;
-    uint32_t acc_phase = 0;
+    uint8_t* boxes = smem_out + (warp - 2) * 2 * kBoxBytes;
     const float alpha = (args.a_g != nullptr ? *args.a_g : 1.f) * (args.b_g != nullptr ? *args.b_g : 1.f);
-    for (int t = blockIdx.x; t < num_tiles; t += gridDim.x) {
-      const int tm = t % num_m, tn = t / num_m;
-      if (!mbar_wait(&tfull[acc], acc_phase, abort_flag, args.err, kErrTimeoutEpilogue)) break;
+    uint32_t release[2];
+    for (int b = 0; b < 2; ++b)
+      release[b] = CTAS == 2 ? map_to_rank(smem_u32(&tempty[b]), 0) : smem_u32(&tempty[b]);
+    int i = 0, box = 0;
+    for (int t = first; t < num_tiles; t += step, ++i) {
+      int tm, tn;
+      tile_at(t, num_m, num_n, tm, tn);
+      const int acc = i & 1;
+      if (!mbar_wait(&tfull[acc], (i >> 1) & 1, abort_flag, args.err, kErrTimeoutEpilogue)) break;
       tc_fence_after();
-      const int row = tm * kBM + q * 32 + lane;
-      T* out = reinterpret_cast<T*>(args.out) + static_cast<long>(row) * args.N;
-      for (int c = 0; c < BN / 32; ++c) {
-        uint32_t r[32];
-        tmem_ld32(tmem + (static_cast<uint32_t>(q * 32) << 16) + acc * BN + 32 * c, r);
-        tmem_wait_ld();
-        if (row < args.M) {
+      const int row0 = (tm * CTAS + rank) * kBM + q * 32;
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const int n = tn * BN + 32 * c + i;
-            if (n < args.N)
-              out[n] = from_float<T>(fmaf(__uint_as_float(r[i]), alpha, args.bias != nullptr ? args.bias[n] : 0.f));
+      for (int step_g = 0; step_g < GROUPS; ++step_g) {
+        // the columns shared with the next accumulator first: the first accumulator's last ones
+        const int g = C::OVERLAP && acc == 0 ? GROUPS - 1 - step_g : step_g;
+        uint32_t r[2][32];
+        const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16) + acc * C::ACC1 + 64 * g;
+        tmem_ld32(taddr, r[0]);
+        tmem_ld32(taddr + 32, r[1]);
+        tmem_wait_ld();
+        if (step_g == (C::OVERLAP ? 0 : GROUPS - 1)) {
+          static_assert(!C::OVERLAP || BN - C::ACC1 <= 64, "shared columns lie in one group");
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) arrive_at(release[acc]);
+        }
+        const int col0 = tn * BN + 64 * g;
+        if (row0 >= args.M || col0 >= args.N) continue;
+        float v[64];
+#pragma unroll
+        for (int j = 0; j < 64; ++j) v[j] = __uint_as_float(r[j / 32][j % 32]) * alpha;
+        if (args.bias != nullptr) {
+#pragma unroll
+          for (int j = 0; j < 64; ++j) v[j] += col0 + j < args.N ? __ldg(args.bias + col0 + j) : 0.f;
+        }
+#pragma unroll
+        for (int h = 0; h < 64 / BOX; ++h) {
+          const int col = col0 + BOX * h;
+          uint8_t* dst = boxes + box * kBoxBytes;
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+          __syncwarp();
+          stage_row<T>(dst, lane, v + BOX * h);
+          if (tma_out) {
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0 && col < args.N) {
+              store_2d(&tmOut, dst, col, row0);
+              bulk_commit_group();
+            }
+          } else {  // rows of no 16-byte pitch: lanes along the row
+            __syncwarp();
+            const int cols = min(BOX, args.N - col);
+            for (int rr = 0; rr < min(32, args.M - row0); ++rr) {
+              T* out = reinterpret_cast<T*>(args.out) + static_cast<long>(row0 + rr) * args.N + col;
+              for (int c = lane; c < cols; c += 32) {
+                const int byte = c * static_cast<int>(sizeof(T));
+                out[c] = *reinterpret_cast<const T*>(dst + rr * 128 + ((byte / 16) ^ (rr & 7)) * 16 + byte % 16);
+              }
+            }
           }
+          box ^= 1;
         }
       }
-      tc_fence_before();
-      mbar_arrive(&tempty[acc]);
-      acc ^= 1;
-      if (acc == 0) acc_phase ^= 1;
     }
+    if (lane == 0) bulk_wait_group_read0();
   }
 
   tc_fence_before();
-  __syncthreads();
+  if constexpr (CTAS == 2) cluster_sync();
+  else __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, C::TMEM_COLS);
+    free_tmem<CTAS>(tmem);
   }
 }
 
-// Codes as a byte matrix [rows, row_bytes], boxes of `box_rows` x 128 bytes.
-CUtensorMap make_codes_map(const void* ptr, long row_bytes, long rows, int box_rows) {
+CUtensorMap encode(CUtensorMapDataType type, int rank, const void* ptr, const cuuint64_t* dims, const cuuint64_t* strides,
+                   const cuuint32_t* box, CUtensorMapSwizzle swizzle, const char* what) {
   CUtensorMap map;
+  const cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = tensor_map_encoder()(&map, type, rank, const_cast<void*>(ptr), dims, strides, box, estr,
+                                          CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  AVGEN_CHECK(r == CUDA_SUCCESS, "mx_gemm: cuTensorMapEncodeTiled failed for ", what, " (", static_cast<int>(r), ")");
+  return map;
+}
+
+// Codes as a byte matrix [rows, row_bytes], boxes of `box_rows` x 128 bytes.
+CUtensorMap codes_map(const void* ptr, long row_bytes, long rows, int box_rows) {
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(row_bytes), static_cast<cuuint64_t>(rows)};
   const cuuint64_t strides[1] = {static_cast<cuuint64_t>(row_bytes)};
   const cuuint32_t box[2] = {kRowBytes, static_cast<cuuint32_t>(box_rows)};
-  const cuuint32_t estr[2] = {1, 1};
-  const CUresult r = tensor_map_encoder()(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides,
-                                          box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  AVGEN_CHECK(r == CUDA_SUCCESS, "mx_gemm: cuTensorMapEncodeTiled failed (", static_cast<int>(r), ")");
-  return map;
+  return encode(CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, ptr, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, "codes");
+}
+
+// Scale tiles as [row groups, tiles, 128 words], boxes of `tiles` tiles of `groups` row groups.
+CUtensorMap scales_map(const void* ptr, long tiles_k, long rows, int tiles, int groups) {
+  const cuuint64_t dims[3] = {128, static_cast<cuuint64_t>(tiles_k), static_cast<cuuint64_t>((rows + 127) / 128)};
+  const cuuint64_t strides[2] = {512, static_cast<cuuint64_t>(tiles_k * 512)};
+  const cuuint32_t box[3] = {128, static_cast<cuuint32_t>(tiles), static_cast<cuuint32_t>(groups)};
+  return encode(CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, ptr, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE, "scales");
+}
+
+template <typename T>
+CUtensorMap out_map(void* ptr, long rows, long cols) {
+  constexpr auto type = sizeof(T) == 4                           ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                        : std::is_same<T, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                                 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(cols) * sizeof(T)};
+  const cuuint32_t box[2] = {128 / sizeof(T), 32};
+  return encode(type, 2, ptr, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, "the output");
+}
+
+template <typename T, int FMT, int BN, int CTAS>
+void launch_tiles(const MxGemmDesc& d, const MxArgs& args, cudaStream_t stream) {
+  using C = Cfg<FMT, BN, CTAS>;
+  const long row_bytes = mx_row_bytes(FMT, d.K), tiles_k = mx_scale_tiles(FMT, d.K);
+  const CUtensorMap ta = codes_map(d.a_codes, row_bytes, d.M, kBM);
+  const CUtensorMap tb = codes_map(d.b_codes, row_bytes, d.N, C::B_ROWS);
+  const CUtensorMap tsa = scales_map(d.a_scales, tiles_k, d.M, C::SF_TILES, 1);
+  const CUtensorMap tsb = scales_map(d.b_scales, tiles_k, d.N, C::SF_TILES, BN / 128);
+  const bool tma_out = static_cast<long>(d.N) * sizeof(T) % 16 == 0;
+  const CUtensorMap to = tma_out ? out_map<T>(d.out, d.M, d.N) : ta;
+  auto kernel = mx_gemm_kernel<T, FMT, BN, CTAS>;
+  static PerDeviceOnce once;
+  raise_smem_limit(once, kernel, C::SMEM_BYTES);
+  const long tiles = static_cast<long>((d.M + CTAS * kBM - 1) / (CTAS * kBM)) * ((d.N + BN - 1) / BN);
+  AVGEN_CHECK(tiles < (1L << 30), "mx_gemm: too many output tiles");
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(CTAS * std::min<long>(tiles, num_sms(d.device) / CTAS)));
+  cfg.blockDim = dim3(192);
+  cfg.dynamicSmemBytes = C::SMEM_BYTES;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = CTAS;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = CTAS == 2 ? 1 : 0;
+  AVGEN_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, ta, tb, tsa, tsb, to, tma_out, args));
 }
 
 template <typename T, int FMT>
 void launch(const MxGemmDesc& d, cudaStream_t stream) {
-  constexpr int BN = 128;
-  using C = Cfg<FMT, BN>;
   MxArgs args{};
-  args.M = d.M, args.N = d.N, args.K = d.K;
-  args.row_bytes = static_cast<int>(mx_row_bytes(FMT, d.K));
-  args.tiles_k = static_cast<int>(mx_scale_tiles(FMT, d.K));
-  args.a_scales = d.a_scales, args.b_scales = d.b_scales;
+  args.M = d.M, args.N = d.N;
+  const long row_bytes = mx_row_bytes(FMT, d.K);
+  args.num_kb = static_cast<int>((row_bytes + kRowBytes - 1) / kRowBytes);
+  args.last_steps = static_cast<int>((row_bytes - static_cast<long>(args.num_kb - 1) * kRowBytes + 31) / 32);
   args.a_g = d.a_g, args.b_g = d.b_g;
   args.bias = d.bias, args.out = d.out, args.err = d.err;
-  const CUtensorMap ta = make_codes_map(d.a_codes, args.row_bytes, d.M, kBM);
-  const CUtensorMap tb = make_codes_map(d.b_codes, args.row_bytes, d.N, BN);
-  auto kernel = mx_gemm_kernel<T, FMT, BN>;
-  static PerDeviceOnce once;
-  raise_smem_limit(once, kernel, C::SMEM_BYTES);
-  const int tiles = (d.M + kBM - 1) / kBM * ((d.N + BN - 1) / BN);
-  kernel<<<std::min(tiles, num_sms(d.device)), 192, C::SMEM_BYTES, stream>>>(ta, tb, args);
-  AVGEN_CUDA_CHECK(cudaGetLastError());
+  const long pair_tiles = static_cast<long>((d.M + 255) / 256) * ((d.N + 255) / 256);
+  if (pair_tiles * 2 >= num_sms(d.device)) return launch_tiles<T, FMT, 256, 2>(d, args, stream);
+  launch_tiles<T, FMT, 128, 1>(d, args, stream);
 }
 
 }  // namespace

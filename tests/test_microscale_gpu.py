@@ -192,7 +192,7 @@ def test_add_rmsnorm_edges() -> None:
 # ----------------------------------------------------------------------------- product
 PRODUCTS = [(1, 1, 1), (1, 8, 32), (2, 130, 65), (128, 128, 256), (129, 127, 96), (200, 300, 1000), (257, 513, 2570),
             (1, 2560, 2560), (16, 640, 4096), (33, 1024, 160), (64, 200, 13824), (640, 384, 129), (1000, 2568, 512),
-            (130, 24, 10240), (3, 7, 30000)]
+            (130, 24, 10240), (3, 7, 30000), (2400, 2100, 160), (4000, 1304, 1100), (300, 20000, 520)]
 
 
 def _check_product(a: mx.MXTensor, b: mx.MXTensor, bias: torch.Tensor | None, dtype: torch.dtype) -> None:
