@@ -998,7 +998,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> mx_add_rmsnorm(const at::Tensor& 
   d.fmt = static_cast<int>(fmt);
   d.dtype = mx_dtype(x.scalar_type(), "add_rmsnorm: x");
   d.rows = rows.size(0);
-  TORCH_CHECK(rows.size(1) <= (1 << 20), "add_rmsnorm: at most ", 1 << 20, " columns, got ", rows.size(1));
+  TORCH_CHECK(rows.size(1) <= kMxNormMaxCols, "add_rmsnorm: at most ", kMxNormMaxCols, " columns, got ", rows.size(1));
   d.W = static_cast<int>(rows.size(1));
   d.eps = static_cast<float>(eps);
   d.x = rows.data_ptr();

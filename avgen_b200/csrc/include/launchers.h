@@ -437,6 +437,7 @@ struct MxNormDesc {
   uint8_t* scales = nullptr;
   const float* g = nullptr;
 };
+constexpr int kMxNormMaxCols = 65536;  // a row stays in one CTA's registers
 void mx_add_rmsnorm_launch(const MxNormDesc& d, cudaStream_t stream);
 
 // out[M, N] = A[M, K] . B[N, K]^T (+ bias), both operands in format `fmt`.
