@@ -948,6 +948,7 @@ std::tuple<at::Tensor, at::Tensor, OptT> mx_quantize(const at::Tensor& x, int64_
   d.rows = rows.size(0);
   d.cols = rows.size(1);
   d.x = rows.data_ptr();
+  TORCH_CHECK(d.rows < (1L << 31) - 256 && d.cols < (1L << 25), "quantize: too many rows or columns");
   d.ldx = rows.stride(0);
   const auto bytes = x.options().dtype(at::kByte);
   at::Tensor codes = at::empty({d.rows, mx_row_bytes(d.fmt, d.cols)}, bytes);
@@ -1002,6 +1003,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> mx_add_rmsnorm(const at::Tensor& 
   d.W = static_cast<int>(rows.size(1));
   d.eps = static_cast<float>(eps);
   d.x = rows.data_ptr();
+  TORCH_CHECK(d.rows < (1L << 31) - 256, "add_rmsnorm: too many rows");
   d.ldx = rows.stride(0);
   at::Tensor u, out = x;
   if (has(update)) {

@@ -65,6 +65,16 @@ __device__ __forceinline__ uint32_t cvt_e4m3x2(float lo, float hi) {
 __device__ __forceinline__ uint32_t cvt_e4m3x4(float a, float b, float c, float d) {
   return cvt_e4m3x2(a, b) | (cvt_e4m3x2(c, d) << 16);
 }
+// Two e2m1 codes, `lo` in the low half of the byte.
+__device__ __forceinline__ uint32_t cvt_e2m1x2(float lo, float hi) {
+  uint32_t r;
+  asm("{\n\t.reg .b8 b0;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+      "mov.b32 %0, {b0, b0, b0, b0};\n\t}"
+      : "=r"(r)
+      : "f"(lo), "f"(hi));
+  return r & 0xffu;
+}
 // Eight e2m1 codes, v[0] in the lowest four bits.
 __device__ __forceinline__ uint32_t cvt_e2m1x8(const float* v) {
   uint32_t r;
@@ -84,6 +94,11 @@ __device__ __forceinline__ float2 e4m3x2_to_float2(uint32_t two) {
   return __half22float2(*reinterpret_cast<__half2*>(&h));
 }
 __device__ __forceinline__ float e4m3_to_float(uint32_t byte) { return e4m3x2_to_float2(byte & 0xffu).x; }
+__device__ __forceinline__ float e2m1_to_float(uint32_t code) {
+  const float a = (code & 6u) != 0u ? __uint_as_float((126u + ((code >> 1) & 3u)) << 23 | (code & 1u) << 22)
+                                    : (code & 1u) * 0.5f;
+  return (code & 8u) != 0u ? -a : a;
+}
 // Values of the eight e2m1 codes of a word.
 __device__ __forceinline__ void e2m1x8_to_float(uint32_t w, float* v) {
   uint32_t h[4];
@@ -110,17 +125,21 @@ __device__ __forceinline__ void e2m1x8_to_float(uint32_t w, float* v) {
 // exponent and a compare of the fraction. s stays within [-126, 126], where 2^s and
 // 2^-s are both normal fp32 numbers and scaling is exact.
 //
-// nvfp4: amax / (6 g) rounded to e4m3; six_g = 6 * g. A block so small that this
-// rounds to zero has all codes zero.
+// nvfp4: amax / (6 g) rounded to e4m3; six_g = 6 * g, inv_six_g its rounded reciprocal. A
+// block so small that this rounds to zero has all codes zero. The quotient is the
+// correctly rounded one (Markstein, IBM J. Res. Dev. 34, 1990): with y = 1 / b rounded,
+// q = a y and the exact remainder r = a - b q, q + r y rounds to a / b; a tiny quotient
+// whose remainder is not exact rounds to zero, one that overflows saturates.
 //
 // A block with an infinity or a NaN gets the NaN scale: whatever its codes, it reads
 // back as NaN, and so does every product it enters.
 template <int FMT>
-__device__ __forceinline__ MxScale mx_scale_of(uint32_t amax, float g, float six_g) {
+__device__ __forceinline__ MxScale mx_scale_of(uint32_t amax, float g, float six_g, float inv_six_g) {
   MxScale r;
   if constexpr (FMT == kNvFp4) {
     if (amax >= kInfBits) return {0x7fu, 0.f};
-    r.byte = cvt_e4m3x2(fminf(__fdiv_rn(__uint_as_float(amax), six_g), 448.f), 0.f) & 0xffu;
+    const float a = __uint_as_float(amax), q = a * inv_six_g;
+    r.byte = cvt_e4m3x2(fminf(fmaf(fmaf(-six_g, q, a), inv_six_g, q), 448.f), 0.f) & 0xffu;
     const float s = e4m3_to_float(r.byte);
     r.inv = r.byte != 0u ? __frcp_rn(s * g) : 0.f;
   } else {

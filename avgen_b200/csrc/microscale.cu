@@ -1,12 +1,12 @@
 // Quantising rows to block-scaled formats, reading them back, and the residual
 // RMSNorm that writes its output quantised.
 //
-// All three are bound by memory. In each, a lane owns 16 consecutive columns of a row
-// (one nvfp4 block, half an mx block) and a warp 512: inputs of aligned rows arrive in
-// 32-byte loads, a block's largest value needs at most one shuffle, the four scales of
-// a tile's row one or two more, and codes leave in 8- or 16-byte stores. Rows of any
-// other alignment pass through shared memory, so that global memory still sees a
-// warp's accesses side by side.
+// All three are bound by memory, quantising to 4 bits also by instruction issue. A lane
+// owns 16 (norm: 8) consecutive columns: a block's largest value takes at most two
+// shuffles, the scales of a tile's row are joined by two, codes leave in one store.
+// Aligned rows are read and written in 16- and 32-byte accesses. Rows of any other
+// alignment are read and written by every 32nd column, so that a warp's accesses still
+// lie side by side, and change layout in shared memory.
 #include <algorithm>
 
 #include "include/host_utils.h"
@@ -17,19 +17,25 @@
 namespace avgen {
 namespace {
 
-constexpr int kLane = 16;         // columns of a lane
-constexpr int kSpan = 32 * kLane; // columns of a warp
+constexpr uint32_t kAllLanes = 0xffffffffu;
 
-// ---------------------------------------------------------------- 16 columns per lane
+// ---------------------------------------------------------------- global memory
+// Inputs are never written by the kernel that reads them (ld.global.nc).
 __device__ __forceinline__ void load32(const void* p, uint32_t* w) {
-  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
-               : "l"(p));
+  asm("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+      : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+      : "l"(p));
+}
+__device__ __forceinline__ void load16(const void* p, uint32_t* w) {
+  asm("ld.global.nc.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(p));
 }
 __device__ __forceinline__ void store32(void* p, const uint32_t* w) {
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
                "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
                : "memory");
+}
+__device__ __forceinline__ void store16(void* p, const uint32_t* w) {
+  *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 template <typename T>
@@ -51,177 +57,285 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   }
 }
 
-// A lane's 16 values as loaded: 8 words of 16-bit values or 16 of fp32.
-template <typename T>
+// abs_bits of the largest magnitude; a NaN among the values gives one (three-input
+// maximum, two values an instruction).
+template <int N>
+__device__ __forceinline__ uint32_t amax_of(const float (&v)[N]) {
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; i += 2)
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(m), "f"(fabsf(v[i])), "f"(fabsf(v[i + 1])));
+  return __float_as_uint(m);
+}
+
+// Two fp32 values in one 64-bit register: one instruction does both.
+struct Pair {
+  unsigned long long b;
+
+  __device__ __forceinline__ Pair(float lo, float hi) { asm("mov.b64 %0, {%1, %2};" : "=l"(b) : "f"(lo), "f"(hi)); }
+  __device__ __forceinline__ void get(float& lo, float& hi) const {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(b));
+  }
+  __device__ __forceinline__ Pair operator*(Pair o) const {
+    Pair r = *this;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.b) : "l"(b), "l"(o.b));
+    return r;
+  }
+  __device__ __forceinline__ Pair operator+(Pair o) const {
+    Pair r = *this;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.b) : "l"(b), "l"(o.b));
+    return r;
+  }
+  // this * o + c
+  __device__ __forceinline__ Pair times_plus(Pair o, Pair c) const {
+    Pair r = *this;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.b) : "l"(b), "l"(o.b), "l"(c.b));
+    return r;
+  }
+};
+
+// v[i] *= s
+template <int N>
+__device__ __forceinline__ void scale_all(float (&v)[N], float s) {
+  const Pair ss(s, s);
+#pragma unroll
+  for (int i = 0; i < N; i += 2) (Pair(v[i], v[i + 1]) * ss).get(v[i], v[i + 1]);
+}
+
+// N values of type T as they lie in memory.
+template <typename T, int N>
 struct Raw {
-  static constexpr int WORDS = kLane * sizeof(T) / 4;
+  static constexpr int WORDS = N * sizeof(T) / 4;
   uint32_t w[WORDS];
 
+  // From / to an address on 32 bytes (or on all of a shorter run).
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (WORDS == 4) {
+      load16(p, w);
+    } else {
+#pragma unroll
+      for (int i = 0; i < WORDS; i += 8) load32(reinterpret_cast<const uint32_t*>(p) + i, w + i);
+    }
+  }
+  __device__ __forceinline__ void store(T* p) const {
+    if constexpr (WORDS == 4) {
+      store16(p, w);
+    } else {
+#pragma unroll
+      for (int i = 0; i < WORDS; i += 8) store32(reinterpret_cast<uint32_t*>(p) + i, w + i);
+    }
+  }
   __device__ __forceinline__ void zero() {
 #pragma unroll
     for (int i = 0; i < WORDS; ++i) w[i] = 0u;
   }
-  __device__ __forceinline__ void unpack(float (&v)[kLane]) const {
+  __device__ __forceinline__ void unpack(float (&v)[N]) const {
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
-      for (int i = 0; i < kLane; ++i) v[i] = __uint_as_float(w[i]);
+      for (int i = 0; i < N; ++i) v[i] = __uint_as_float(w[i]);
     } else {
 #pragma unroll
-      for (int i = 0; i < kLane / 2; ++i) unpack2<T>(w[i], v[2 * i], v[2 * i + 1]);
+      for (int i = 0; i < N / 2; ++i) unpack2<T>(w[i], v[2 * i], v[2 * i + 1]);
     }
   }
-  __device__ __forceinline__ void pack(const float (&v)[kLane]) {
+  __device__ __forceinline__ void pack(const float (&v)[N]) {
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
-      for (int i = 0; i < kLane; ++i) w[i] = __float_as_uint(v[i]);
+      for (int i = 0; i < N; ++i) w[i] = __float_as_uint(v[i]);
     } else {
 #pragma unroll
-      for (int i = 0; i < kLane / 2; ++i) w[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
+      for (int i = 0; i < N / 2; ++i) w[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
+    }
+  }
+  // abs_bits of the largest magnitude. 16-bit values are compared two at a time by their
+  // own bits, which order like theirs as fp32.
+  __device__ __forceinline__ uint32_t amax() const {
+    if constexpr (sizeof(T) == 4) {
+      float v[N];
+      unpack(v);
+      return amax_of(v);
+    } else {
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < WORDS; i += 2)
+        m = __vimax3_u16x2(m, w[i] & 0x7fff7fffu, w[i + 1] & 0x7fff7fffu);
+      const uint32_t top = max(m & 0xffffu, m >> 16);
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) return top << 16;
+      return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(top))));
     }
   }
 };
 
-// Columns [c0, c0 + 16) of a row of `cols`, zero past its end; `c0` = the warp's first
-// column + 16 * lane, `stage` 16 * 32 values of shared memory of the warp's own.
-// Called by whole warps.
-template <typename T, bool ALIGNED>
-__device__ __forceinline__ void load16(const T* row, long c0, long cols, uint32_t* stage, Raw<T>& r) {
-  if constexpr (ALIGNED) {  // cols is a multiple of 16
-    if (c0 < cols) {
-#pragma unroll
-      for (int i = 0; i < Raw<T>::WORDS; i += 8) load32(reinterpret_cast<const uint32_t*>(row + c0) + i, r.w + i);
-    } else {
-      r.zero();
-    }
-  } else {
-    T* s = reinterpret_cast<T*>(stage);
-    const int lane = lane_id();
-    const long base = c0 - kLane * lane;
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < kLane; ++i) {
-      const long c = base + 32 * i + lane;
-      s[32 * i + lane] = c < cols ? row[c] : from_float<T>(0.f);
-    }
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < Raw<T>::WORDS; i += 4)
-      *reinterpret_cast<uint4*>(r.w + i) = *reinterpret_cast<const uint4*>(stage + lane * Raw<T>::WORDS + i);
-  }
-}
-template <typename T, bool ALIGNED>
-__device__ __forceinline__ void store16(T* row, long c0, long cols, uint32_t* stage, const Raw<T>& r) {
-  if constexpr (ALIGNED) {
-    if (c0 < cols) {
-#pragma unroll
-      for (int i = 0; i < Raw<T>::WORDS; i += 8) store32(reinterpret_cast<uint32_t*>(row + c0) + i, r.w + i);
-    }
-  } else {
-    const T* s = reinterpret_cast<const T*>(stage);
-    const int lane = lane_id();
-    const long base = c0 - kLane * lane;
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < Raw<T>::WORDS; i += 4)
-      *reinterpret_cast<uint4*>(stage + lane * Raw<T>::WORDS + i) = *reinterpret_cast<const uint4*>(r.w + i);
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < kLane; ++i) {
-      const long c = base + 32 * i + lane;
-      if (c < cols) row[c] = s[32 * i + lane];
-    }
-  }
-}
-
-// Where a packed row goes.
+// ---------------------------------------------------------------- packed rows
 struct PackedRows {
   uint8_t* codes;
   uint8_t* scales;
   long row_bytes;
   long tiles;
   long cols;
+
+  __device__ __forceinline__ uint8_t* codes_of(long row) const { return codes + row * row_bytes; }
+  // The scales of a row's first tile.
+  __device__ __forceinline__ uint8_t* scales_of(long row) const {
+    const uint32_t r = static_cast<uint32_t>(row);
+    return scales + static_cast<long>(r >> 7) * (tiles * 512) + (r & 31u) * 16 + (r >> 5 & 3u) * 4;
+  }
 };
 
-// Quantises and stores a lane's 16 values (zero past the row's end). Called by whole warps.
-template <int FMT>
-__device__ __forceinline__ void store_packed(const PackedRows& p, long row, long c0, float (&v)[kLane], float g,
-                                             float six_g) {
-  constexpr int B = mx_block(FMT);
-  constexpr int LANES = B / kLane;  // lanes of a block
-  const int lane = lane_id();
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < kLane; ++i) m = max(m, abs_bits(v[i]));
-  if constexpr (LANES == 2) m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-  const MxScale s = mx_scale_of<FMT>(m, g, six_g);
-  uint32_t word = (c0 & ~static_cast<long>(B - 1)) < p.cols ? s.byte << (8 * (lane / LANES & 3)) : 0u;
-  word |= __shfl_xor_sync(0xffffffffu, word, LANES);
-  word |= __shfl_xor_sync(0xffffffffu, word, 2 * LANES);
-  const long tile = c0 / (4 * B);
-  if (lane % (4 * LANES) == 0 && tile < p.tiles)
-    *reinterpret_cast<uint32_t*>(p.scales + mx_scale_word(row, tile, p.tiles)) = word;
-  const long at = c0 * mx_bits(FMT) / 8;
-  if (at >= p.row_bytes) return;
-#pragma unroll
-  for (int i = 0; i < kLane; ++i) v[i] *= s.inv;
-  uint8_t* out = p.codes + row * p.row_bytes + at;
-  if constexpr (FMT == kMxFp8) {
-    *reinterpret_cast<uint4*>(out) =
-        make_uint4(cvt_e4m3x4(v[0], v[1], v[2], v[3]), cvt_e4m3x4(v[4], v[5], v[6], v[7]),
-                   cvt_e4m3x4(v[8], v[9], v[10], v[11]), cvt_e4m3x4(v[12], v[13], v[14], v[15]));
-  } else {
-    *reinterpret_cast<uint2*>(out) = make_uint2(cvt_e2m1x8(v), cvt_e2m1x8(v + 8));
+// What a lane with the N columns from c0 (a multiple of N) stores in every row. Lanes of a
+// warp lie side by side.
+template <int FMT, int N>
+struct LanePlace {
+  static constexpr int B = mx_block(FMT);
+  static constexpr int LANES = B / N;  // lanes of a block
+  uint32_t code_at;   // offset of its codes, or past any row
+  uint32_t scale_at;  // offset of the scale word it writes, or past any tile
+  uint32_t byte_mask; // its block's place in that word, or none
+
+  __device__ __forceinline__ LanePlace(const PackedRows& p, long c0) {
+    const int lane = lane_id();
+    const long at = c0 * mx_bits(FMT) / 8, tile = c0 / (4 * B);
+    code_at = at < p.row_bytes ? static_cast<uint32_t>(at) : ~0u;
+    scale_at = lane % (4 * LANES) == 0 && tile < p.tiles ? static_cast<uint32_t>(tile * 512) : ~0u;
+    byte_mask = (c0 & ~static_cast<long>(B - 1)) < p.cols ? 0xffu << (8 * (lane / LANES & 3)) : 0u;
   }
+};
+
+// Quantises and stores a lane's N values (zero past the row's end), whose largest
+// magnitude is `m`. Called by whole warps.
+template <int FMT, int N>
+__device__ __forceinline__ void store_packed(const LanePlace<FMT, N>& at, uint8_t* codes, uint8_t* scales, float (&v)[N],
+                                             uint32_t m, float g, float six_g, float inv_six_g) {
+  constexpr int LANES = LanePlace<FMT, N>::LANES;
+  if constexpr (LANES >= 2) m = max(m, __shfl_xor_sync(kAllLanes, m, 1));
+  if constexpr (LANES >= 4) m = max(m, __shfl_xor_sync(kAllLanes, m, 2));
+  const MxScale s = mx_scale_of<FMT>(m, g, six_g, inv_six_g);
+  uint32_t word = (s.byte * 0x01010101u) & at.byte_mask;
+  word |= __shfl_xor_sync(kAllLanes, word, LANES);
+  word |= __shfl_xor_sync(kAllLanes, word, 2 * LANES);
+  if (at.scale_at != ~0u) *reinterpret_cast<uint32_t*>(scales + at.scale_at) = word;
+  if (at.code_at == ~0u) return;
+  scale_all(v, s.inv);
+  constexpr int WORDS = N * mx_bits(FMT) / 32;
+  uint32_t w[WORDS];
+#pragma unroll
+  for (int i = 0; i < WORDS; ++i) {
+    if constexpr (FMT == kMxFp8) w[i] = cvt_e4m3x4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    else w[i] = cvt_e2m1x8(v + 8 * i);
+  }
+  uint32_t* out = reinterpret_cast<uint32_t*>(codes + at.code_at);
+  if constexpr (WORDS == 4) *reinterpret_cast<uint4*>(out) = make_uint4(w[0], w[1], w[2], w[3]);
+  else if constexpr (WORDS == 2) *reinterpret_cast<uint2*>(out) = make_uint2(w[0], w[1]);
+  else *out = w[0];
 }
+
 // The (zero) scales of a row past the tensor, inside its last 128-row group.
 __device__ __forceinline__ void store_pad_scales(const PackedRows& p, long row, long first_tile, long end_tile, int lane,
                                                  int lanes) {
   for (long t = first_tile + lane; t < min(end_tile, p.tiles); t += lanes)
-    *reinterpret_cast<uint32_t*>(p.scales + mx_scale_word(row, t, p.tiles)) = 0u;
+    *reinterpret_cast<uint32_t*>(p.scales_of(row) + t * 512) = 0u;
 }
 
 // ---------------------------------------------------------------- quantise
-// Largest finite |value| of a lane's 16, as bits.
-template <typename T>
-__device__ __forceinline__ uint32_t finite_amax(const Raw<T>& r) {
-  float v[kLane];
-  r.unpack(v);
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < kLane; ++i) {
-    const uint32_t b = abs_bits(v[i]);
-    m = max(m, b < kInfBits ? b : 0u);
-  }
-  return m;
-}
+constexpr int kLane = 16;          // columns of a lane
+constexpr int kSpan = 32 * kLane;  // columns of a warp
 
-// The tensor scale's pass: atomicMax of whole numbers, so the order does not matter.
-template <typename T, bool ALIGNED>
-__global__ void __launch_bounds__(256) mx_amax_kernel(MxQuantDesc d, int segments) {
-  __shared__ __align__(16) uint32_t stage[ALIGNED ? 1 : 8][kSpan * sizeof(T) / 4];
-  const int warp = warp_id(), lane = lane_id();
-  const long units = d.rows * segments;  // of one row x 512 columns
-  uint32_t m = 0;
-  for (long u = blockIdx.x * 8L + warp; u < units; u += gridDim.x * 8L) {
-    const long row = u / segments;
-    Raw<T> r;
-    load16<T, ALIGNED>(reinterpret_cast<const T*>(d.x) + row * d.ldx, (u - row * segments) * kSpan + lane * kLane, d.cols,
-                       stage[ALIGNED ? 0 : warp], r);
-    m = max(m, finite_amax(r));
+// 512 columns of an unaligned row: read side by side, handed to the lanes that own them
+// through the warp's `stage`, and back.
+template <typename T>
+struct Unaligned {
+  T v[kLane];  // columns base + 32 j + lane
+
+  __device__ __forceinline__ void load(const T* row, long base, long cols) {
+#pragma unroll
+    for (int j = 0; j < kLane; ++j) {
+      const long c = base + 32 * j + lane_id();
+      v[j] = c < cols ? row[c] : from_float<T>(0.f);
+    }
   }
-  m = __reduce_max_sync(0xffffffffu, m);
+  __device__ __forceinline__ void to_lanes(T* stage, Raw<T, kLane>& r) const {
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < kLane; ++j) stage[32 * j + lane_id()] = v[j];
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < r.WORDS; i += 4)
+      *reinterpret_cast<uint4*>(r.w + i) = reinterpret_cast<const uint4*>(stage + lane_id() * kLane)[i / 4];
+  }
+  static __device__ __forceinline__ void store(T* row, long base, long cols, T* stage, const Raw<T, kLane>& r) {
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < r.WORDS; i += 4)
+      reinterpret_cast<uint4*>(stage + lane_id() * kLane)[i / 4] = *reinterpret_cast<const uint4*>(r.w + i);
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < kLane; ++j) {
+      const long c = base + 32 * j + lane_id();
+      if (c < cols) row[c] = stage[32 * j + lane_id()];
+    }
+  }
+};
+
+// The tensor scale's pass: the largest finite |value|. atomicMax of whole numbers, so
+// the order does not matter.
+template <typename T, bool ALIGNED>
+__global__ void __launch_bounds__(256) mx_amax_kernel(MxQuantDesc d) {
+  constexpr int UNROLL = ALIGNED ? 4 : 1;
+  const int lane = lane_id();
+  const long base = static_cast<long>(blockIdx.y) * kSpan;
+  const long c0 = base + lane * kLane;
+  const long step = gridDim.x * 8L;
+  uint32_t m = 0;
+  auto keep_finite = [&](const float* v) {
+#pragma unroll
+    for (int i = 0; i < kLane; ++i) {
+      const uint32_t b = abs_bits(v[i]);
+      m = max(m, b < kInfBits ? b : 0u);
+    }
+  };
+  for (long row = blockIdx.x * 8L + warp_id(); row < d.rows; row += UNROLL * step) {
+    if constexpr (ALIGNED) {
+      Raw<T, kLane> r[UNROLL];
+#pragma unroll
+      for (int i = 0; i < UNROLL; ++i) {
+        const long at = row + i * step;
+        if (at < d.rows && c0 < d.cols) r[i].load(reinterpret_cast<const T*>(d.x) + at * d.ldx + c0);
+        else r[i].zero();
+      }
+#pragma unroll
+      for (int i = 0; i < UNROLL; ++i) {
+        const uint32_t b = r[i].amax();
+        if (b < kInfBits) {
+          m = max(m, b);
+        } else {
+          float v[kLane];
+          r[i].unpack(v);
+          keep_finite(v);
+        }
+      }
+    } else {
+      Unaligned<T> u;
+      u.load(reinterpret_cast<const T*>(d.x) + row * d.ldx, base, d.cols);
+      float v[kLane];
+#pragma unroll
+      for (int i = 0; i < kLane; ++i) v[i] = to_float(u.v[i]);
+      keep_finite(v);
+    }
+  }
+  m = __reduce_max_sync(kAllLanes, m);
   if (lane == 0 && m != 0u) atomicMax(d.amax, m);
 }
 
 // A CTA quantises `rows_per_cta` rows x 512 columns, a warp one row at a time.
 template <typename T, int FMT, bool ALIGNED>
 __global__ void __launch_bounds__(256) mx_quantize_kernel(MxQuantDesc d, PackedRows p, int rows_per_cta) {
-  __shared__ __align__(16) uint32_t stage[ALIGNED ? 1 : 8][kSpan * sizeof(T) / 4];
-  constexpr int UNROLL = ALIGNED ? (sizeof(T) == 2 ? 4 : 2) : 1;
+  constexpr int UNROLL = ALIGNED && sizeof(T) == 2 ? 4 : 2;
+  __shared__ __align__(16) T stage[ALIGNED ? 1 : 8][ALIGNED ? 8 : kSpan];
   const int warp = warp_id(), lane = lane_id();
   // nvfp4 has just read the whole tensor for its scale: from the end, where L2 still holds it
   const long group = FMT == kNvFp4 ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
-  const long c0 = static_cast<long>(blockIdx.y) * kSpan + lane * kLane;
+  const long base = static_cast<long>(blockIdx.y) * kSpan;
+  const long c0 = base + lane * kLane;
   float g = 1.f;
   if constexpr (FMT == kNvFp4) {
     if (d.amax != nullptr) {
@@ -231,15 +345,22 @@ __global__ void __launch_bounds__(256) mx_quantize_kernel(MxQuantDesc d, PackedR
       g = *d.g;
     }
   }
-  const float six_g = 6.f * g;
+  const float six_g = 6.f * g, inv_six_g = __frcp_rn(six_g);
+  const LanePlace<FMT, kLane> place(p, c0);
   const long end = min((d.rows + 127) / 128 * 128, (group + 1) * rows_per_cta);
   for (long row = group * rows_per_cta + warp; row < end; row += 8 * UNROLL) {
-    Raw<T> r[UNROLL];
+    Raw<T, kLane> r[UNROLL];
+    Unaligned<T> u[ALIGNED ? 1 : UNROLL];
 #pragma unroll
     for (int i = 0; i < UNROLL; ++i) {
       const long at = row + 8 * i;
-      if (at < min(end, d.rows))
-        load16<T, ALIGNED>(reinterpret_cast<const T*>(d.x) + at * d.ldx, c0, d.cols, stage[ALIGNED ? 0 : warp], r[i]);
+      const T* x = reinterpret_cast<const T*>(d.x) + at * d.ldx;
+      if constexpr (ALIGNED) {
+        if (at < min(end, d.rows) && c0 < d.cols) r[i].load(x + c0);
+        else r[i].zero();
+      } else if (at < min(end, d.rows)) {
+        u[i].load(x, base, d.cols);
+      }
     }
 #pragma unroll
     for (int i = 0; i < UNROLL; ++i) {
@@ -247,8 +368,9 @@ __global__ void __launch_bounds__(256) mx_quantize_kernel(MxQuantDesc d, PackedR
       if (at >= end) break;
       if (at < d.rows) {
         float v[kLane];
+        if constexpr (!ALIGNED) u[i].to_lanes(stage[warp], r[i]);
         r[i].unpack(v);
-        store_packed<FMT>(p, at, c0, v, g, six_g);
+        store_packed<FMT>(place, p.codes_of(at), p.scales_of(at), v, r[i].amax(), g, six_g, inv_six_g);
       } else {
         constexpr int TILES = kSpan / (4 * mx_block(FMT));
         store_pad_scales(p, at, static_cast<long>(blockIdx.y) * TILES, static_cast<long>(blockIdx.y + 1) * TILES, lane, 32);
@@ -260,151 +382,230 @@ __global__ void __launch_bounds__(256) mx_quantize_kernel(MxQuantDesc d, PackedR
 // ---------------------------------------------------------------- read back
 template <typename T, int FMT, bool ALIGNED>
 __global__ void __launch_bounds__(256) mx_dequantize_kernel(MxDequantDesc d, PackedRows p, int rows_per_cta) {
-  __shared__ __align__(16) uint32_t stage[ALIGNED ? 1 : 8][kSpan * sizeof(T) / 4];
   constexpr int B = mx_block(FMT);
   constexpr int WORDS = kLane * mx_bits(FMT) / 32;
-  constexpr int UNROLL = 4;
+  constexpr int UNROLL = ALIGNED ? 4 : 2;
+  __shared__ __align__(16) T stage[ALIGNED ? 1 : 8][ALIGNED ? 8 : kSpan];
   const int warp = warp_id(), lane = lane_id();
-  const long c0 = static_cast<long>(blockIdx.y) * kSpan + lane * kLane;
+  const long base = static_cast<long>(blockIdx.y) * kSpan;
+  const long c0 = base + lane * kLane;
   const float g = FMT == kNvFp4 && d.g != nullptr ? *d.g : 1.f;
   const long end = min(d.rows, (blockIdx.x + 1L) * rows_per_cta);
   const long at = c0 * mx_bits(FMT) / 8;
+  const long scale_at = c0 / (4 * B) * 512 + c0 / B % 4;
   const bool inside = c0 < d.cols;
   for (long row = static_cast<long>(blockIdx.x) * rows_per_cta + warp; row < end; row += 8 * UNROLL) {
-    uint32_t w[UNROLL][WORDS], sb[UNROLL];
+    uint32_t w[UNROLL][WORDS] = {}, sb[UNROLL] = {};
 #pragma unroll
     for (int i = 0; i < UNROLL; ++i) {
       const long r = row + 8 * i;
       if (r < end && inside) {
-        const uint32_t* in = reinterpret_cast<const uint32_t*>(p.codes + r * p.row_bytes + at);
-        if constexpr (WORDS == 4) *reinterpret_cast<uint4*>(w[i]) = *reinterpret_cast<const uint4*>(in);
-        else *reinterpret_cast<uint2*>(w[i]) = *reinterpret_cast<const uint2*>(in);
-        sb[i] = p.scales[mx_scale_word(r, c0 / (4 * B), p.tiles) + c0 / B % 4];
+        const uint32_t* in = reinterpret_cast<const uint32_t*>(p.codes_of(r) + at);
+        if constexpr (WORDS == 4) *reinterpret_cast<uint4*>(w[i]) = __ldg(reinterpret_cast<const uint4*>(in));
+        else *reinterpret_cast<uint2*>(w[i]) = __ldg(reinterpret_cast<const uint2*>(in));
+        sb[i] = __ldg(p.scales_of(r) + scale_at);
       }
     }
 #pragma unroll
     for (int i = 0; i < UNROLL; ++i) {
       const long r = row + 8 * i;
       if (r >= end) break;
+      if (ALIGNED && !inside) break;
       float v[kLane];
-      Raw<T> out;
-      if (inside) {
-        const float s = mx_scale_value<FMT>(sb[i]);
-        if constexpr (FMT == kMxFp8) {
+      const float s = mx_scale_value<FMT>(sb[i]);
+      if constexpr (FMT == kMxFp8) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float2 lo = e4m3x2_to_float2(w[i][j] & 0xffffu), hi = e4m3x2_to_float2(w[i][j] >> 16);
-            v[4 * j] = lo.x * s, v[4 * j + 1] = lo.y * s, v[4 * j + 2] = hi.x * s, v[4 * j + 3] = hi.y * s;
-          }
-        } else {
-          e2m1x8_to_float(w[i][0], v);
-          e2m1x8_to_float(w[i][1], v + 8);
-#pragma unroll
-          for (int j = 0; j < kLane; ++j) v[j] = FMT == kNvFp4 ? v[j] * s * g : v[j] * s;
+        for (int j = 0; j < 4; ++j) {
+          const float2 lo = e4m3x2_to_float2(w[i][j] & 0xffffu), hi = e4m3x2_to_float2(w[i][j] >> 16);
+          v[4 * j] = lo.x, v[4 * j + 1] = lo.y, v[4 * j + 2] = hi.x, v[4 * j + 3] = hi.y;
         }
-        out.pack(v);
+      } else {
+        e2m1x8_to_float(w[i][0], v);
+        e2m1x8_to_float(w[i][1], v + 8);
       }
-      store16<T, ALIGNED>(reinterpret_cast<T*>(d.out) + r * d.cols, c0, d.cols, stage[ALIGNED ? 0 : warp], out);
+      scale_all(v, s);
+      if constexpr (FMT == kNvFp4) scale_all(v, g);
+      Raw<T, kLane> out;
+      out.pack(v);
+      T* dst = reinterpret_cast<T*>(d.out) + r * d.cols;
+      if constexpr (ALIGNED) out.store(dst + c0);
+      else Unaligned<T>::store(dst, base, d.cols, stage[warp], out);
     }
   }
 }
 
 // ---------------------------------------------------------------- residual RMSNorm
-// A CTA takes one row at a time, CHUNKS pieces of 16 columns per lane held in
-// registers between the sum of squares and the store: x and the update are read once.
-// The norm takes the fp32 sum x + gate * update, not its rounding to T; statistics,
-// modulation and scaling stay in fp32 until the codes.
-template <typename T, int FMT, int CHUNKS, bool ALIGNED>
-__global__ void __launch_bounds__(CHUNKS == 4 ? 1024 : 512) mx_add_rmsnorm_kernel(MxNormDesc d, PackedRows p) {
-  extern __shared__ __align__(16) uint32_t stages[];  // 512 fp32 per warp where rows are not aligned
-  __shared__ float red[2][32];
-  const int warp = warp_id(), lane = lane_id(), warps = blockDim.x >> 5;
-  uint32_t* stage = ALIGNED ? nullptr : stages + warp * kSpan;
-  const float g = FMT == kNvFp4 && d.g != nullptr ? *d.g : 1.f;
-  const float six_g = 6.f * g;
-  const long padded = (d.rows + 127) / 128 * 128;
-  int turn = 0;
-  for (long row = blockIdx.x; row < padded; row += gridDim.x) {
-    if (row >= d.rows) {
-      store_pad_scales(p, row, 0, p.tiles, threadIdx.x, blockDim.x);
-      continue;
-    }
-    float v[CHUNKS][kLane];
-    const T* x = reinterpret_cast<const T*>(d.x) + row * d.ldx;
-    const long b = d.num_groups > 0 ? mod_row(d.groups, d.num_groups, row, d.rows_per_batch) : 0;
-    float ss = 0.f;
+constexpr int kNormLane = 8;  // columns of a lane in one chunk: fp32 modulation rows in 32-byte loads side by side
+constexpr int kNormSpan = 32 * kNormLane;
+
+// Eight columns per lane of the 256-column chunk at `base`: consecutive ones of an
+// aligned row, every 32nd of any other.
+template <typename T, bool ALIGNED>
+struct Chunk {
+  Raw<T, kNormLane> r;
+
+  __device__ __forceinline__ void load(const T* row, int base, int cols) {
+    const int lane = lane_id();
+    if constexpr (ALIGNED) {
+      const int c = base + lane * kNormLane;
+      if (c < cols) r.load(row + c);
+      else r.zero();
+    } else {
+      float v[kNormLane];
 #pragma unroll
-    for (int i = 0; i < CHUNKS; ++i) {
-      const long c0 = static_cast<long>(i * warps + warp) * kSpan + lane * kLane;
-      Raw<T> rx, ru;
-      load16<T, ALIGNED>(x, c0, d.W, stage, rx);
-      if (d.update != nullptr)
-        load16<T, ALIGNED>(reinterpret_cast<const T*>(d.update) + row * d.ldu, c0, d.W, stage, ru);
-      rx.unpack(v[i]);
-      if (d.update != nullptr) {
-        float u[kLane];
-        ru.unpack(u);
-        if (d.gate != nullptr) {
-          Raw<float> t;
-          load16<float, ALIGNED>(d.gate + b * d.gate_stride, c0, d.W, stage, t);
-#pragma unroll
-          for (int e = 0; e < kLane; ++e) v[i][e] = fmaf(__uint_as_float(t.w[e]), u[e], v[i][e]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < kLane; ++e) v[i][e] += u[e];
-        }
-        rx.pack(v[i]);
-        store16<T, ALIGNED>(reinterpret_cast<T*>(d.x_out) + row * d.W, c0, d.W, stage, rx);
+      for (int e = 0; e < kNormLane; ++e) {
+        const int c = base + 32 * e + lane;
+        v[e] = c < cols ? to_float(row[c]) : 0.f;
       }
-#pragma unroll
-      for (int e = 0; e < kLane; ++e) ss = fmaf(v[i][e], v[i][e], ss);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if (lane == 0) red[turn][warp] = ss;
-    __syncthreads();  // one per row: the next row's sums go to the other buffer
-    ss = 0.f;
-    for (int i = 0; i < warps; ++i) ss += red[turn][i];
-    turn ^= 1;
-    const float r = rsqrtf(ss / static_cast<float>(d.W) + d.eps);
-#pragma unroll
-    for (int i = 0; i < CHUNKS; ++i) {
-      const long c0 = static_cast<long>(i * warps + warp) * kSpan + lane * kLane;
-      Raw<float> t;
-#pragma unroll
-      for (int e = 0; e < kLane; ++e) v[i][e] *= r;
-      if (d.w != nullptr) {
-        load16<float, ALIGNED>(d.w, c0, d.W, stage, t);
-#pragma unroll
-        for (int e = 0; e < kLane; ++e) v[i][e] *= __uint_as_float(t.w[e]);
-      }
-      if (d.scale != nullptr) {
-        load16<float, ALIGNED>(d.scale + b * d.mod_stride, c0, d.W, stage, t);
-#pragma unroll
-        for (int e = 0; e < kLane; ++e) v[i][e] *= 1.f + __uint_as_float(t.w[e]);
-      }
-      if (d.shift != nullptr) {
-        load16<float, ALIGNED>(d.shift + b * d.mod_stride, c0, d.W, stage, t);
-#pragma unroll
-        for (int e = 0; e < kLane; ++e) v[i][e] += __uint_as_float(t.w[e]);
-      }
-      if (c0 >= d.W) {  // 0 * (a statistic that overflowed) is not 0
-#pragma unroll
-        for (int e = 0; e < kLane; ++e) v[i][e] = 0.f;
-      } else if (!ALIGNED) {
-#pragma unroll
-        for (int e = 0; e < kLane; ++e) v[i][e] = c0 + e < d.W ? v[i][e] : 0.f;
-      }
-      store_packed<FMT>(p, row, c0, v[i], g, six_g);
+      r.pack(v);
     }
   }
+  __device__ __forceinline__ void store(T* row, int base, int cols) const {
+    const int lane = lane_id();
+    if constexpr (ALIGNED) {
+      const int c = base + lane * kNormLane;
+      if (c < cols) r.store(row + c);
+    } else {
+      float v[kNormLane];
+      r.unpack(v);
+#pragma unroll
+      for (int e = 0; e < kNormLane; ++e) {
+        const int c = base + 32 * e + lane;
+        if (c < cols) row[c] = from_float<T>(v[e]);
+      }
+    }
+  }
+  __device__ __forceinline__ Pair pair(int e) const { return {__uint_as_float(r.w[e]), __uint_as_float(r.w[e + 1])}; }
+};
+
+// A row is held in registers, CHUNKS x 8 columns per lane, between its sum of squares
+// and its store: x and the update are read once. Rows of up to 1024 columns take one
+// warp each (WARP_ROWS) and no barrier; longer ones a CTA, with one barrier per row. The
+// next row's x and update are requested before the reduction, so that loads stay in
+// flight through it.
+//
+// The norm takes the fp32 sum x + gate * update, not its rounding to T; statistics,
+// modulation and scaling stay in fp32 until the codes.
+template <typename T, int FMT, int CHUNKS, bool WARP_ROWS, bool ALIGNED>
+__global__ void __launch_bounds__(CHUNKS == 8 ? 1024 : 512) mx_add_rmsnorm_kernel(MxNormDesc d, PackedRows p) {
+  extern __shared__ __align__(16) float stages[];  // 256 per warp, unaligned rows only
+  __shared__ float red[2][32];
+  const int warp = warp_id(), lane = lane_id();
+  const int warps = WARP_ROWS ? 1 : blockDim.x >> 5;  // of a row
+  const int place = WARP_ROWS ? 0 : warp;
+  const float g = FMT == kNvFp4 && d.g != nullptr ? *d.g : 1.f;
+  const float six_g = 6.f * g, inv_six_g = __frcp_rn(six_g), inv_w = 1.f / static_cast<float>(d.W);
+  const int padded = static_cast<int>((d.rows + 127) / 128 * 128), rows = static_cast<int>(d.rows);
+  const int step = WARP_ROWS ? gridDim.x * (blockDim.x >> 5) : gridDim.x;
+  int row = WARP_ROWS ? blockIdx.x * (blockDim.x >> 5) + warp : blockIdx.x;
+  const int base = place * kNormSpan, stride = warps * kNormSpan;  // of the warp's chunks
+
+  Chunk<T, ALIGNED> rx[CHUNKS], ru[CHUNKS];
+  int next_b = 0;
+  auto request = [&](int at) {
+    if (d.num_groups > 0) next_b = static_cast<int>(mod_row(d.groups, d.num_groups, at, d.rows_per_batch));
+    const T* x = reinterpret_cast<const T*>(d.x) + at * d.ldx;
+    const T* u = reinterpret_cast<const T*>(d.update) + at * d.ldu;
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i) {
+      rx[i].load(x, base + i * stride, d.W);
+      if (d.update != nullptr) ru[i].load(u, base + i * stride, d.W);
+    }
+  };
+  if (row < rows) request(row);
+  int turn = 0;
+  for (; row < rows; row += step) {
+    float v[CHUNKS][kNormLane];
+    const float* gate = d.gate + next_b * d.gate_stride;
+    const float* scale = d.scale + next_b * d.mod_stride;
+    const float* shift = d.shift + next_b * d.mod_stride;
+    T* x_out = reinterpret_cast<T*>(d.x_out) + static_cast<long>(row) * d.W;
+    Pair ss(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i) {
+      Chunk<float, ALIGNED> t;
+      if (d.gate != nullptr) t.load(gate, base + i * stride, d.W);
+      rx[i].r.unpack(v[i]);
+      if (d.update != nullptr) {
+        float u[kNormLane];
+        ru[i].r.unpack(u);
+#pragma unroll
+        for (int e = 0; e < kNormLane; e += 2) {
+          const Pair x2(v[i][e], v[i][e + 1]), u2(u[e], u[e + 1]);
+          (d.gate != nullptr ? t.pair(e).times_plus(u2, x2) : x2 + u2).get(v[i][e], v[i][e + 1]);
+        }
+        rx[i].r.pack(v[i]);
+        rx[i].store(x_out, base + i * stride, d.W);
+      }
+#pragma unroll
+      for (int e = 0; e < kNormLane; e += 2) {
+        const Pair x2(v[i][e], v[i][e + 1]);
+        ss = x2.times_plus(x2, ss);
+      }
+    }
+    if (row + step < rows) request(row + step);
+    float sum, other;
+    ss.get(sum, other);
+    sum += other;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kAllLanes, sum, o);
+    if constexpr (!WARP_ROWS) {
+      if (lane == 0) red[turn][warp] = sum;
+      __syncthreads();  // one per row: the next row's sums go to the other buffer
+      sum = 0.f;
+      for (int i = 0; i < warps; ++i) sum += red[turn][i];
+      turn ^= 1;
+    }
+    const float r = rsqrtf(fmaf(sum, inv_w, d.eps));
+    uint8_t* codes = p.codes_of(row);
+    uint8_t* scales = p.scales_of(row);
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i) {
+      const int at = base + i * stride;
+      Chunk<float, ALIGNED> t;
+      scale_all(v[i], r);
+      if (d.w != nullptr) {
+        t.load(d.w, at, d.W);
+#pragma unroll
+        for (int e = 0; e < kNormLane; e += 2) (Pair(v[i][e], v[i][e + 1]) * t.pair(e)).get(v[i][e], v[i][e + 1]);
+      }
+      if (d.scale != nullptr) {
+        t.load(scale, at, d.W);
+#pragma unroll
+        for (int e = 0; e < kNormLane; e += 2)
+          (Pair(v[i][e], v[i][e + 1]) * (t.pair(e) + Pair(1.f, 1.f))).get(v[i][e], v[i][e + 1]);
+      }
+      if (d.shift != nullptr) {
+        t.load(shift, at, d.W);
+#pragma unroll
+        for (int e = 0; e < kNormLane; e += 2) (Pair(v[i][e], v[i][e + 1]) + t.pair(e)).get(v[i][e], v[i][e + 1]);
+      }
+      const int c0 = at + lane * kNormLane;
+      if constexpr (!ALIGNED) {
+        float* stage = stages + warp * kNormSpan;
+        __syncwarp();
+#pragma unroll
+        for (int e = 0; e < kNormLane; ++e) stage[32 * e + lane] = v[i][e];
+        __syncwarp();
+#pragma unroll
+        for (int e = 0; e < kNormLane; ++e) v[i][e] = c0 + e < d.W ? stage[lane * kNormLane + e] : 0.f;
+      } else if (c0 >= d.W) {  // 0 * (a statistic that overflowed) is not 0
+#pragma unroll
+        for (int e = 0; e < kNormLane; ++e) v[i][e] = 0.f;
+      }
+      store_packed<FMT>(LanePlace<FMT, kNormLane>(p, c0), codes, scales, v[i], amax_of(v[i]), g, six_g, inv_six_g);
+    }
+  }
+  for (; row < padded; row += step)
+    store_pad_scales(p, row, 0, p.tiles, WARP_ROWS ? lane : threadIdx.x, WARP_ROWS ? 32 : blockDim.x);
 }
 
 // ---------------------------------------------------------------- launches
 bool aligned32(const void* ptr) { return reinterpret_cast<uintptr_t>(ptr) % 32 == 0; }
-// Whether rows of `cols` values of `size` bytes, `ld` values apart, all start on 32 bytes and end on 16 values.
-bool rows_aligned(const void* ptr, long rows, long ld, long cols, int size) {
-  return aligned32(ptr) && cols % kLane == 0 && (rows <= 1 || ld * size % 32 == 0);
+// Whether rows of `cols` values of `size` bytes, `ld` values apart, all start on 32 bytes
+// and end on a lane's run of `lane` values.
+bool rows_aligned(const void* ptr, long rows, long ld, long cols, int size, int lane) {
+  return aligned32(ptr) && cols % lane == 0 && (rows <= 1 || ld * size % std::min(32, lane * size) == 0);
 }
 
 // Rows of a CTA: as many as leave four CTAs for every SM (fewer, larger CTAs keep the
@@ -422,8 +623,9 @@ void quantize_as(const MxQuantDesc& d, const PackedRows& p, cudaStream_t stream)
   const int sms = num_sms(d.device);
   if (d.amax != nullptr) {
     AVGEN_CUDA_CHECK(cudaMemsetAsync(d.amax, 0, sizeof(uint32_t), stream));
-    const long blocks = std::min<long>((d.rows * segments + 31) / 32, 8L * sms);
-    mx_amax_kernel<T, ALIGNED><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(d, static_cast<int>(segments));
+    const long blocks = std::min<long>((d.rows + 31) / 32, std::max<long>(1, 8L * sms / segments));
+    mx_amax_kernel<T, ALIGNED>
+        <<<dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(segments)), 256, 0, stream>>>(d);
   }
   const long rows = (d.rows + 127) / 128 * 128;
   const int rpc = rows_per_cta(d.rows, segments, sms);
@@ -435,7 +637,7 @@ void quantize_as(const MxQuantDesc& d, const PackedRows& p, cudaStream_t stream)
 template <typename T, int FMT>
 void quantize(const MxQuantDesc& d, cudaStream_t stream) {
   const PackedRows p{d.codes, d.scales, mx_row_bytes(FMT, d.cols), mx_scale_tiles(FMT, d.cols), d.cols};
-  if (rows_aligned(d.x, d.rows, d.ldx, d.cols, sizeof(T))) quantize_as<T, FMT, true>(d, p, stream);
+  if (rows_aligned(d.x, d.rows, d.ldx, d.cols, sizeof(T), kLane)) quantize_as<T, FMT, true>(d, p, stream);
   else quantize_as<T, FMT, false>(d, p, stream);
 }
 
@@ -453,28 +655,30 @@ template <typename T, int FMT>
 void dequantize(const MxDequantDesc& d, cudaStream_t stream) {
   const PackedRows p{const_cast<uint8_t*>(d.codes), const_cast<uint8_t*>(d.scales), mx_row_bytes(FMT, d.cols),
                      mx_scale_tiles(FMT, d.cols), d.cols};
-  if (rows_aligned(d.out, d.rows, d.cols, d.cols, sizeof(T))) dequantize_as<T, FMT, true>(d, p, stream);
+  if (rows_aligned(d.out, d.rows, d.cols, d.cols, sizeof(T), kLane)) dequantize_as<T, FMT, true>(d, p, stream);
   else dequantize_as<T, FMT, false>(d, p, stream);
 }
 
-template <typename T, int FMT, int CHUNKS, bool ALIGNED>
+template <typename T, int FMT, int CHUNKS, bool WARP_ROWS, bool ALIGNED>
 void add_rmsnorm_as(const MxNormDesc& d, const PackedRows& p, int warps, cudaStream_t stream) {
-  auto kernel = mx_add_rmsnorm_kernel<T, FMT, CHUNKS, ALIGNED>;
-  const int smem = ALIGNED ? 0 : warps * kSpan * 4;
-  static PerDeviceOnce once;
-  if (!ALIGNED) raise_smem_limit(once, kernel, 32 * kSpan * 4);
+  auto kernel = mx_add_rmsnorm_kernel<T, FMT, CHUNKS, WARP_ROWS, ALIGNED>;
   const long padded = (d.rows + 127) / 128 * 128;
+  const long units = WARP_ROWS ? (padded + warps - 1) / warps : padded;
   const long ctas = static_cast<long>(std::max(1, 64 / warps)) * num_sms(d.device);
-  kernel<<<static_cast<unsigned>(std::min(padded, ctas)), 32 * warps, smem, stream>>>(d, p);
+  const int smem = ALIGNED ? 0 : warps * kNormSpan * 4;  // at most 32 KB
+  kernel<<<static_cast<unsigned>(std::min(units, ctas)), 32 * warps, smem, stream>>>(d, p);
   AVGEN_CUDA_CHECK(cudaGetLastError());
 }
 
 template <typename T, int FMT, bool ALIGNED>
 void add_rmsnorm_aligned(const MxNormDesc& d, const PackedRows& p, cudaStream_t stream) {
-  const int spans = static_cast<int>(std::max<long>((d.W + kSpan - 1) / kSpan, 1));
-  if (spans <= 8) return add_rmsnorm_as<T, FMT, 1, ALIGNED>(d, p, spans, stream);
-  if (spans <= 32) return add_rmsnorm_as<T, FMT, 2, ALIGNED>(d, p, (spans + 1) / 2, stream);
-  add_rmsnorm_as<T, FMT, 4, ALIGNED>(d, p, (spans + 3) / 4, stream);
+  const int spans = static_cast<int>((d.W + kNormSpan - 1) / kNormSpan);
+  if (spans == 1) return add_rmsnorm_as<T, FMT, 1, true, ALIGNED>(d, p, 4, stream);
+  if (spans == 2) return add_rmsnorm_as<T, FMT, 2, true, ALIGNED>(d, p, 4, stream);
+  if (spans <= 4) return add_rmsnorm_as<T, FMT, 4, true, ALIGNED>(d, p, 4, stream);
+  if (spans <= 32) return add_rmsnorm_as<T, FMT, 2, false, ALIGNED>(d, p, (spans + 1) / 2, stream);
+  if (spans <= 64) return add_rmsnorm_as<T, FMT, 4, false, ALIGNED>(d, p, (spans + 3) / 4, stream);
+  add_rmsnorm_as<T, FMT, 8, false, ALIGNED>(d, p, (spans + 7) / 8, stream);
 }
 
 template <typename T, int FMT>
@@ -482,9 +686,8 @@ void add_rmsnorm(const MxNormDesc& d, cudaStream_t stream) {
   AVGEN_CHECK(d.W <= kMxNormMaxCols, "add_rmsnorm: at most ", kMxNormMaxCols, " columns, got ", d.W);
   const PackedRows p{d.codes, d.scales, mx_row_bytes(FMT, d.W), mx_scale_tiles(FMT, d.W), d.W};
   auto mod = [&](const float* t, long stride) { return t == nullptr || (aligned32(t) && stride % 8 == 0); };
-  const bool aligned = rows_aligned(d.x, d.rows, d.ldx, d.W, sizeof(T)) &&
-                       (d.update == nullptr || (rows_aligned(d.update, d.rows, d.ldu, d.W, sizeof(T)) &&
-                                                rows_aligned(d.x_out, d.rows, d.W, d.W, sizeof(T)))) &&
+  auto rows = [&](const void* t, long ld) { return rows_aligned(t, d.rows, ld, d.W, sizeof(T), kNormLane); };
+  const bool aligned = rows(d.x, d.ldx) && (d.update == nullptr || (rows(d.update, d.ldu) && rows(d.x_out, d.W))) &&
                        mod(d.w, 0) && mod(d.scale, d.mod_stride) && mod(d.shift, d.mod_stride) &&
                        mod(d.gate, d.gate_stride);
   if (aligned) add_rmsnorm_aligned<T, FMT, true>(d, p, stream);
