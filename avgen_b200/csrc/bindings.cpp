@@ -4,6 +4,7 @@
 // dtype, shape, strides, alignment) and fills the torch-free launch descriptors
 // of include/launchers.h. Kernels run on torch's current CUDA stream.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -900,6 +901,10 @@ void p2p_copy_py(int64_t dst, int64_t src, int64_t bytes) {
 }
 
 // --------------------------------------------------------------------- block-scaled formats
+// Straight to the caching allocator: the dispatcher's share of at::empty counts beside kernels of a few microseconds.
+at::Tensor mx_empty(at::IntArrayRef sizes, at::ScalarType type, at::Device device) {
+  return at::detail::empty_cuda(sizes, type, device, c10::nullopt);
+}
 int mx_dtype(at::ScalarType t, const char* what) {
   if (t == at::kBFloat16) return kMxBf16;
   if (t == at::kHalf) return kMxFp16;
@@ -936,7 +941,8 @@ at::Tensor mx_rows(const at::Tensor& x, const char* name) {
   return cols > 1 && r.stride(1) != 1 ? r.contiguous() : r;
 }
 
-std::tuple<at::Tensor, at::Tensor, OptT> mx_quantize(const at::Tensor& x, int64_t fmt, const OptT& g, bool measure) {
+// (codes, scales, tensor scale or none, kernels launched)
+std::tuple<at::Tensor, at::Tensor, OptT, int> mx_quantize(const at::Tensor& x, int64_t fmt, const OptT& g, bool measure) {
   check_cuda(x, "quantize: x");
   c10::cuda::CUDAGuard guard(x.device());
   const at::Tensor rows = mx_rows(x, "quantize: x");
@@ -950,22 +956,27 @@ std::tuple<at::Tensor, at::Tensor, OptT> mx_quantize(const at::Tensor& x, int64_
   d.x = rows.data_ptr();
   TORCH_CHECK(d.rows < (1L << 31) - 256 && d.cols < (1L << 25), "quantize: too many rows or columns");
   d.ldx = rows.stride(0);
-  const auto bytes = x.options().dtype(at::kByte);
-  at::Tensor codes = at::empty({d.rows, mx_row_bytes(d.fmt, d.cols)}, bytes);
-  at::Tensor scales = at::empty({mx_scale_bytes(d.fmt, d.rows, d.cols)}, bytes);
+  at::Tensor codes = mx_empty({d.rows, mx_row_bytes(d.fmt, d.cols)}, at::kByte, x.device());
+  at::Tensor scales = mx_empty({mx_scale_bytes(d.fmt, d.rows, d.cols)}, at::kByte, x.device());
   d.codes = codes.data_ptr<uint8_t>();
   d.scales = scales.data_ptr<uint8_t>();
   d.g = mx_global(g, x, "quantize: global_scale");
   OptT g_out = g;
+  at::Tensor partial;
   if (fmt == kNvFp4 && measure) {
-    at::Tensor buf = at::empty({2}, x.options().dtype(at::kFloat));
-    if (d.rows == 0) buf.fill_(1.f);
-    g_out = buf.narrow(0, 0, 1);
-    d.g_out = buf.data_ptr<float>();
-    d.amax = reinterpret_cast<unsigned*>(buf.data_ptr<float>() + 1);
+    at::Tensor made = mx_empty({1}, at::kFloat, x.device());
+    if (d.rows == 0) made.fill_(1.f);
+    d.g_out = made.data_ptr<float>();
+    g_out = made;
+    const int parts = mx_quantize_parts(d);
+    if (parts > 0) {
+      partial = mx_empty({parts}, at::kInt, x.device());
+      d.amax = reinterpret_cast<unsigned*>(partial.data_ptr<int>());
+      d.parts = parts;
+    }
   }
   if (d.rows > 0) mx_quantize_launch(d, cur_stream());
-  return {codes, scales, g_out};
+  return {codes, scales, g_out, d.rows == 0 ? 0 : d.parts > 0 ? 2 : 1};
 }
 
 at::Tensor mx_dequantize(const at::Tensor& codes, const at::Tensor& scales, int64_t fmt, int64_t cols, const OptT& g,
@@ -980,7 +991,7 @@ at::Tensor mx_dequantize(const at::Tensor& codes, const at::Tensor& scales, int6
   d.codes = codes.data_ptr<uint8_t>();
   d.scales = scales.data_ptr<uint8_t>();
   d.g = mx_global(g, codes, "dequantize: global_scale");
-  at::Tensor out = at::empty({d.rows, cols}, codes.options().dtype(dtype));
+  at::Tensor out = mx_empty({d.rows, cols}, dtype, codes.device());
   d.out = out.data_ptr();
   if (d.rows > 0) mx_dequantize_launch(d, cur_stream());
   return out;
@@ -1012,7 +1023,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> mx_add_rmsnorm(const at::Tensor& 
     u = mx_rows(*update, "add_rmsnorm: update");
     d.update = u.data_ptr();
     d.ldu = u.stride(0);
-    out = at::empty(x.sizes(), x.options());
+    out = mx_empty(x.sizes(), x.scalar_type(), x.device());
     d.x_out = out.data_ptr();
   }
   d.rows_per_batch = std::max<int64_t>(1, rows_per_batch);
@@ -1047,9 +1058,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> mx_add_rmsnorm(const at::Tensor& 
     TORCH_CHECK(d.groups != nullptr || mod_rows * d.rows_per_batch >= d.rows,
                 "add_rmsnorm: modulation rows do not cover x");
   }
-  const auto bytes = x.options().dtype(at::kByte);
-  at::Tensor codes = at::empty({d.rows, mx_row_bytes(d.fmt, d.W)}, bytes);
-  at::Tensor scales = at::empty({mx_scale_bytes(d.fmt, d.rows, d.W)}, bytes);
+  at::Tensor codes = mx_empty({d.rows, mx_row_bytes(d.fmt, d.W)}, at::kByte, x.device());
+  at::Tensor scales = mx_empty({mx_scale_bytes(d.fmt, d.rows, d.W)}, at::kByte, x.device());
   d.codes = codes.data_ptr<uint8_t>();
   d.scales = scales.data_ptr<uint8_t>();
   if (d.rows > 0) mx_add_rmsnorm_launch(d, cur_stream());
@@ -1080,7 +1090,7 @@ at::Tensor mx_gemm(const at::Tensor& a_codes, const at::Tensor& a_scales, const 
   d.bias = f32_or_null(bias, "matmul: bias");
   TORCH_CHECK(d.bias == nullptr || (bias->numel() == n && bias->device() == a_codes.device()),
               "matmul: bias must be fp32 [", n, "] on the operands' device");
-  at::Tensor out = at::empty({m, n}, a_codes.options().dtype(dtype));
+  at::Tensor out = mx_empty({m, n}, dtype, a_codes.device());
   d.out = out.data_ptr();
   d.err = error_word(d.device);
   if (m > 0 && n > 0) mx_gemm_launch(d, cur_stream());

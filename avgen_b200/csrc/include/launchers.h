@@ -393,9 +393,13 @@ struct MxQuantDesc {
   uint8_t* codes = nullptr;   // [rows, mx_row_bytes]
   uint8_t* scales = nullptr;  // [mx_scale_bytes]
   const float* g = nullptr;   // nvfp4: the caller's tensor scale, or
-  unsigned* amax = nullptr;   // scratch word from which one is made, stored in
-  float* g_out = nullptr;
+  float* g_out = nullptr;     // where one made from the tensor goes,
+  unsigned* amax = nullptr;   // with scratch of `parts` words, each of which the
+  int parts = 0;              // measuring pass writes
 };
+// Scratch words a measured nvfp4 tensor scale needs (rows, cols and device set); 0 where
+// one launch measures and quantises.
+int mx_quantize_parts(const MxQuantDesc& d);
 void mx_quantize_launch(const MxQuantDesc& d, cudaStream_t stream);
 
 struct MxDequantDesc {

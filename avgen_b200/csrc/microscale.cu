@@ -26,8 +26,18 @@ __device__ __forceinline__ void load32(const void* p, uint32_t* w) {
       : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
       : "l"(p));
 }
-__device__ __forceinline__ void load16(const void* p, uint32_t* w) {
-  asm("ld.global.nc.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(p));
+// As load32 where `on`, else the words keep what they hold: a load without a branch.
+__device__ __forceinline__ void load32_if(bool on, const void* p, uint32_t* w) {
+  asm("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %9, 0;\n\t"
+      "@q ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n\t}"
+      : "+r"(w[0]), "+r"(w[1]), "+r"(w[2]), "+r"(w[3]), "+r"(w[4]), "+r"(w[5]), "+r"(w[6]), "+r"(w[7])
+      : "l"(p), "r"(static_cast<int>(on)));
+}
+__device__ __forceinline__ void load16_if(bool on, const void* p, uint32_t* w) {
+  asm("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q ld.global.nc.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}"
+      : "+r"(w[0]), "+r"(w[1]), "+r"(w[2]), "+r"(w[3])
+      : "l"(p), "r"(static_cast<int>(on)));
 }
 __device__ __forceinline__ void store32(void* p, const uint32_t* w) {
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
@@ -110,11 +120,16 @@ struct Raw {
 
   // From / to an address on 32 bytes (or on all of a shorter run).
   __device__ __forceinline__ void load(const T* p) {
+    static_assert(WORDS % 8 == 0, "whole 32-byte loads");
+#pragma unroll
+    for (int i = 0; i < WORDS; i += 8) load32(reinterpret_cast<const uint32_t*>(p) + i, w + i);
+  }
+  __device__ __forceinline__ void load_if(bool on, const T* p) {
     if constexpr (WORDS == 4) {
-      load16(p, w);
+      load16_if(on, p, w);
     } else {
 #pragma unroll
-      for (int i = 0; i < WORDS; i += 8) load32(reinterpret_cast<const uint32_t*>(p) + i, w + i);
+      for (int i = 0; i < WORDS; i += 8) load32_if(on, reinterpret_cast<const uint32_t*>(p) + i, w + i);
     }
   }
   __device__ __forceinline__ void store(T* p) const {
@@ -276,8 +291,27 @@ struct Unaligned {
   }
 };
 
-// The tensor scale's pass: the largest finite |value|. atomicMax of whole numbers, so
-// the order does not matter.
+__device__ __forceinline__ uint32_t finite_max(const float (&v)[kLane]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < kLane; ++i) {
+    const uint32_t b = abs_bits(v[i]);
+    m = max(m, b < kInfBits ? b : 0u);
+  }
+  return m;
+}
+// The same, a few instructions where all values are finite.
+template <typename T>
+__device__ __forceinline__ uint32_t finite_max(const Raw<T, kLane>& r) {
+  const uint32_t m = r.amax();
+  if (m < kInfBits) return m;
+  float v[kLane];
+  r.unpack(v);
+  return finite_max(v);
+}
+
+// The tensor scale's pass: each CTA writes the largest finite |value| it saw, and the
+// quantising CTAs take the maximum of those words.
 template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(256) mx_amax_kernel(MxQuantDesc d) {
   constexpr int UNROLL = ALIGNED ? 4 : 1;
@@ -285,14 +319,8 @@ __global__ void __launch_bounds__(256) mx_amax_kernel(MxQuantDesc d) {
   const long base = static_cast<long>(blockIdx.y) * kSpan;
   const long c0 = base + lane * kLane;
   const long step = gridDim.x * 8L;
+  __shared__ uint32_t warp_max[8];
   uint32_t m = 0;
-  auto keep_finite = [&](const float* v) {
-#pragma unroll
-    for (int i = 0; i < kLane; ++i) {
-      const uint32_t b = abs_bits(v[i]);
-      m = max(m, b < kInfBits ? b : 0u);
-    }
-  };
   for (long row = blockIdx.x * 8L + warp_id(); row < d.rows; row += UNROLL * step) {
     if constexpr (ALIGNED) {
       Raw<T, kLane> r[UNROLL];
@@ -303,27 +331,23 @@ __global__ void __launch_bounds__(256) mx_amax_kernel(MxQuantDesc d) {
         else r[i].zero();
       }
 #pragma unroll
-      for (int i = 0; i < UNROLL; ++i) {
-        const uint32_t b = r[i].amax();
-        if (b < kInfBits) {
-          m = max(m, b);
-        } else {
-          float v[kLane];
-          r[i].unpack(v);
-          keep_finite(v);
-        }
-      }
+      for (int i = 0; i < UNROLL; ++i) m = max(m, finite_max(r[i]));
     } else {
       Unaligned<T> u;
       u.load(reinterpret_cast<const T*>(d.x) + row * d.ldx, base, d.cols);
       float v[kLane];
 #pragma unroll
       for (int i = 0; i < kLane; ++i) v[i] = to_float(u.v[i]);
-      keep_finite(v);
+      m = max(m, finite_max(v));
     }
   }
   m = __reduce_max_sync(kAllLanes, m);
-  if (lane == 0 && m != 0u) atomicMax(d.amax, m);
+  if (lane == 0) warp_max[warp_id()] = m;
+  __syncthreads();
+  if (warp_id() == 0) {
+    m = __reduce_max_sync(kAllLanes, lane < 8 ? warp_max[lane] : 0u);
+    if (lane == 0) d.amax[blockIdx.y * gridDim.x + blockIdx.x] = m;
+  }
 }
 
 // A CTA quantises `rows_per_cta` rows x 512 columns, a warp one row at a time.
@@ -339,7 +363,13 @@ __global__ void __launch_bounds__(256) mx_quantize_kernel(MxQuantDesc d, PackedR
   float g = 1.f;
   if constexpr (FMT == kNvFp4) {
     if (d.amax != nullptr) {
-      g = nvfp4_tensor_scale(*d.amax);
+      __shared__ uint32_t warp_max[8];
+      uint32_t m = 0;
+      for (int i = threadIdx.x; i < d.parts; i += 256) m = max(m, d.amax[i]);
+      m = __reduce_max_sync(kAllLanes, m);
+      if (lane == 0) warp_max[warp] = m;
+      __syncthreads();
+      g = nvfp4_tensor_scale(__reduce_max_sync(kAllLanes, warp_max[lane & 7]));
       if (group == 0 && blockIdx.y == 0 && threadIdx.x == 0) *d.g_out = g;
     } else if (d.g != nullptr) {
       g = *d.g;
@@ -377,6 +407,57 @@ __global__ void __launch_bounds__(256) mx_quantize_kernel(MxQuantDesc d, PackedR
       }
     }
   }
+}
+
+// Small nvfp4 tensors in one launch of one cluster: every warp holds one row x 512
+// columns while the CTAs exchange their maxima.
+constexpr int kSmallWarps = 16, kSmallCtas = 8;
+
+template <typename T, bool ALIGNED>
+__global__ void __launch_bounds__(32 * kSmallWarps) mx_quantize_small_kernel(MxQuantDesc d, PackedRows p, int segments) {
+  __shared__ __align__(16) T stage[ALIGNED ? 1 : kSmallWarps][ALIGNED ? 8 : kSpan];
+  __shared__ uint32_t warp_max[kSmallWarps];
+  __shared__ uint32_t cta_max[kSmallCtas];  // every CTA writes its word in every CTA
+  const int warp = warp_id(), lane = lane_id(), ctas = gridDim.x;
+  const int unit = blockIdx.x * kSmallWarps + warp;
+  const long row = unit / segments, base = static_cast<long>(unit % segments) * kSpan, c0 = base + lane * kLane;
+  const T* x = reinterpret_cast<const T*>(d.x) + row * d.ldx;
+  Raw<T, kLane> r;
+  r.zero();
+  if (row < d.rows) {
+    if constexpr (ALIGNED) {
+      if (c0 < d.cols) r.load(x + c0);
+    } else {
+      Unaligned<T> u;
+      u.load(x, base, d.cols);
+      u.to_lanes(stage[warp], r);
+    }
+  }
+  const uint32_t m = __reduce_max_sync(kAllLanes, finite_max(r));
+  if (lane == 0) warp_max[warp] = m;
+  __syncthreads();
+  if (warp == 0) {
+    const uint32_t all = __reduce_max_sync(kAllLanes, warp_max[lane % kSmallWarps]);
+    if (lane < ctas) {
+      uint32_t at;  // of this CTA's word in CTA `lane`
+      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(&cta_max[blockIdx.x])), "r"(lane));
+      asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(all) : "memory");
+    }
+  }
+  // the scales past the tensor meanwhile
+  const long pad = (p.tiles * ((d.rows + 127) / 128 * 128 - d.rows));
+  for (long i = blockIdx.x * blockDim.x + threadIdx.x; i < pad; i += static_cast<long>(ctas) * blockDim.x)
+    *reinterpret_cast<uint32_t*>(p.scales_of(d.rows + i / p.tiles) + i % p.tiles * 512) = 0u;
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  const float g = nvfp4_tensor_scale(__reduce_max_sync(kAllLanes, lane < ctas ? cta_max[lane % kSmallCtas] : 0u));
+  if (blockIdx.x == 0 && threadIdx.x == 0) *d.g_out = g;
+  if (row >= d.rows) return;
+  float v[kLane];
+  r.unpack(v);
+  const float six_g = 6.f * g;
+  store_packed<kNvFp4>(LanePlace<kNvFp4, kLane>(p, c0), p.codes_of(row), p.scales_of(row), v, r.amax(), g, six_g,
+                       __frcp_rn(six_g));
 }
 
 // ---------------------------------------------------------------- read back
@@ -444,18 +525,22 @@ template <typename T, bool ALIGNED>
 struct Chunk {
   Raw<T, kNormLane> r;
 
-  __device__ __forceinline__ void load(const T* row, int base, int cols) {
+  // `other` past the row's end, and everywhere when there is no such row.
+  __device__ __forceinline__ void load(const T* row, int base, int cols, float other = 0.f) {
     const int lane = lane_id();
+    float v[kNormLane];
     if constexpr (ALIGNED) {
       const int c = base + lane * kNormLane;
-      if (c < cols) r.load(row + c);
-      else r.zero();
+#pragma unroll
+      for (int e = 0; e < kNormLane; ++e) v[e] = other;
+      r.pack(v);
+      r.load_if(row != nullptr && c < cols, row + c);
     } else {
-      float v[kNormLane];
+      const int end = row != nullptr ? cols : 0;
 #pragma unroll
       for (int e = 0; e < kNormLane; ++e) {
         const int c = base + 32 * e + lane;
-        v[e] = c < cols ? to_float(row[c]) : 0.f;
+        v[e] = c < end ? to_float(row[c]) : other;
       }
       r.pack(v);
     }
@@ -500,47 +585,45 @@ __global__ void __launch_bounds__(CHUNKS == 8 ? 1024 : 512) mx_add_rmsnorm_kerne
   int row = WARP_ROWS ? blockIdx.x * (blockDim.x >> 5) + warp : blockIdx.x;
   const int base = place * kNormSpan, stride = warps * kNormSpan;  // of the warp's chunks
 
+  // A missing update, gate, weight, scale or shift reads as 0, 1, 1, 0 and 0: no branches, so loads are issued together.
   Chunk<T, ALIGNED> rx[CHUNKS], ru[CHUNKS];
   int next_b = 0;
   auto request = [&](int at) {
     if (d.num_groups > 0) next_b = static_cast<int>(mod_row(d.groups, d.num_groups, at, d.rows_per_batch));
     const T* x = reinterpret_cast<const T*>(d.x) + at * d.ldx;
-    const T* u = reinterpret_cast<const T*>(d.update) + at * d.ldu;
+    const T* u = d.update != nullptr ? reinterpret_cast<const T*>(d.update) + at * d.ldu : nullptr;
 #pragma unroll
     for (int i = 0; i < CHUNKS; ++i) {
       rx[i].load(x, base + i * stride, d.W);
-      if (d.update != nullptr) ru[i].load(u, base + i * stride, d.W);
+      ru[i].load(u, base + i * stride, d.W);
     }
   };
+  auto level = [](const float* t, long at) { return t != nullptr ? t + at : nullptr; };
   if (row < rows) request(row);
   int turn = 0;
   for (; row < rows; row += step) {
     float v[CHUNKS][kNormLane];
-    const float* gate = d.gate + next_b * d.gate_stride;
-    const float* scale = d.scale + next_b * d.mod_stride;
-    const float* shift = d.shift + next_b * d.mod_stride;
+    const float* gate = level(d.gate, next_b * d.gate_stride);
+    const float* scale = level(d.scale, next_b * d.mod_stride);
+    const float* shift = level(d.shift, next_b * d.mod_stride);
     T* x_out = reinterpret_cast<T*>(d.x_out) + static_cast<long>(row) * d.W;
     Pair ss(0.f, 0.f);
 #pragma unroll
     for (int i = 0; i < CHUNKS; ++i) {
       Chunk<float, ALIGNED> t;
-      if (d.gate != nullptr) t.load(gate, base + i * stride, d.W);
+      t.load(gate, base + i * stride, d.W, 1.f);
+      float u[kNormLane];
       rx[i].r.unpack(v[i]);
-      if (d.update != nullptr) {
-        float u[kNormLane];
-        ru[i].r.unpack(u);
-#pragma unroll
-        for (int e = 0; e < kNormLane; e += 2) {
-          const Pair x2(v[i][e], v[i][e + 1]), u2(u[e], u[e + 1]);
-          (d.gate != nullptr ? t.pair(e).times_plus(u2, x2) : x2 + u2).get(v[i][e], v[i][e + 1]);
-        }
-        rx[i].r.pack(v[i]);
-        rx[i].store(x_out, base + i * stride, d.W);
-      }
+      ru[i].r.unpack(u);
 #pragma unroll
       for (int e = 0; e < kNormLane; e += 2) {
-        const Pair x2(v[i][e], v[i][e + 1]);
+        const Pair x2 = t.pair(e).times_plus(Pair(u[e], u[e + 1]), Pair(v[i][e], v[i][e + 1]));
+        x2.get(v[i][e], v[i][e + 1]);
         ss = x2.times_plus(x2, ss);
+      }
+      if (d.x_out != nullptr) {
+        rx[i].r.pack(v[i]);
+        rx[i].store(x_out, base + i * stride, d.W);
       }
     }
     if (row + step < rows) request(row + step);
@@ -562,23 +645,15 @@ __global__ void __launch_bounds__(CHUNKS == 8 ? 1024 : 512) mx_add_rmsnorm_kerne
 #pragma unroll
     for (int i = 0; i < CHUNKS; ++i) {
       const int at = base + i * stride;
-      Chunk<float, ALIGNED> t;
-      scale_all(v[i], r);
-      if (d.w != nullptr) {
-        t.load(d.w, at, d.W);
+      Chunk<float, ALIGNED> w, sc, sh;
+      w.load(d.w, at, d.W, 1.f);
+      sc.load(scale, at, d.W);
+      sh.load(shift, at, d.W);
+      const Pair r2(r, r), one(1.f, 1.f);
 #pragma unroll
-        for (int e = 0; e < kNormLane; e += 2) (Pair(v[i][e], v[i][e + 1]) * t.pair(e)).get(v[i][e], v[i][e + 1]);
-      }
-      if (d.scale != nullptr) {
-        t.load(scale, at, d.W);
-#pragma unroll
-        for (int e = 0; e < kNormLane; e += 2)
-          (Pair(v[i][e], v[i][e + 1]) * (t.pair(e) + Pair(1.f, 1.f))).get(v[i][e], v[i][e + 1]);
-      }
-      if (d.shift != nullptr) {
-        t.load(shift, at, d.W);
-#pragma unroll
-        for (int e = 0; e < kNormLane; e += 2) (Pair(v[i][e], v[i][e + 1]) + t.pair(e)).get(v[i][e], v[i][e + 1]);
+      for (int e = 0; e < kNormLane; e += 2) {
+        const Pair y = Pair(v[i][e], v[i][e + 1]) * r2 * w.pair(e);
+        y.times_plus(sc.pair(e) + one, sh.pair(e)).get(v[i][e], v[i][e + 1]);
       }
       const int c0 = at + lane * kNormLane;
       if constexpr (!ALIGNED) {
@@ -616,19 +691,33 @@ int rows_per_cta(long rows, long segments, int sms) {
   return 8;
 }
 
+long segments_of(long cols) { return (cols + kSpan - 1) / kSpan; }
+
 template <typename T, int FMT, bool ALIGNED>
 void quantize_as(const MxQuantDesc& d, const PackedRows& p, cudaStream_t stream) {
-  const long segments = (p.tiles * 4 * mx_block(FMT) + kSpan - 1) / kSpan;
+  const long segments = segments_of(d.cols);
   AVGEN_CHECK(segments <= 65535, "quantize: too many columns: ", d.cols);
-  const int sms = num_sms(d.device);
-  if (d.amax != nullptr) {
-    AVGEN_CUDA_CHECK(cudaMemsetAsync(d.amax, 0, sizeof(uint32_t), stream));
-    const long blocks = std::min<long>((d.rows + 31) / 32, std::max<long>(1, 8L * sms / segments));
-    mx_amax_kernel<T, ALIGNED>
-        <<<dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(segments)), 256, 0, stream>>>(d);
+  if constexpr (FMT == kNvFp4) {
+    if (d.g_out != nullptr && d.amax == nullptr) {
+      cudaLaunchConfig_t cfg{};
+      cfg.gridDim = dim3(static_cast<unsigned>((d.rows * segments + kSmallWarps - 1) / kSmallWarps));
+      cfg.blockDim = dim3(32 * kSmallWarps);
+      cfg.stream = stream;
+      cudaLaunchAttribute attr{};
+      attr.id = cudaLaunchAttributeClusterDimension;
+      attr.val.clusterDim.x = cfg.gridDim.x;
+      attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+      cfg.attrs = &attr;
+      cfg.numAttrs = 1;
+      AVGEN_CUDA_CHECK(cudaLaunchKernelEx(&cfg, mx_quantize_small_kernel<T, ALIGNED>, d, p, static_cast<int>(segments)));
+      return;
+    }
+    if (d.amax != nullptr)
+      mx_amax_kernel<T, ALIGNED>
+          <<<dim3(static_cast<unsigned>(d.parts / segments), static_cast<unsigned>(segments)), 256, 0, stream>>>(d);
   }
   const long rows = (d.rows + 127) / 128 * 128;
-  const int rpc = rows_per_cta(d.rows, segments, sms);
+  const int rpc = rows_per_cta(d.rows, segments, num_sms(d.device));
   mx_quantize_kernel<T, FMT, ALIGNED>
       <<<dim3(static_cast<unsigned>(rows / rpc), static_cast<unsigned>(segments)), 256, 0, stream>>>(d, p, rpc);
   AVGEN_CUDA_CHECK(cudaGetLastError());
@@ -643,7 +732,7 @@ void quantize(const MxQuantDesc& d, cudaStream_t stream) {
 
 template <typename T, int FMT, bool ALIGNED>
 void dequantize_as(const MxDequantDesc& d, const PackedRows& p, cudaStream_t stream) {
-  const long segments = (d.cols + kSpan - 1) / kSpan;
+  const long segments = segments_of(d.cols);
   AVGEN_CHECK(segments <= 65535, "dequantize: too many columns: ", d.cols);
   const int rpc = rows_per_cta(d.rows, segments, num_sms(d.device));
   mx_dequantize_kernel<T, FMT, ALIGNED>
@@ -709,6 +798,14 @@ void add_rmsnorm(const MxNormDesc& d, cudaStream_t stream) {
     if ((d).dtype == kMxFp32 && (d).fmt == kNvFp4) return what<float, kNvFp4>(d, stream);         \
     AVGEN_CHECK(false, #what ": unsupported type ", (d).dtype, " or format ", (d).fmt);           \
   } while (0)
+
+int mx_quantize_parts(const MxQuantDesc& d) {
+  const long segments = segments_of(d.cols);
+  if (d.rows * segments <= kSmallWarps * kSmallCtas) return 0;
+  // CTAs of the measuring pass: up to eight for every SM, 32 rows of 512 columns at least
+  const long blocks = std::min<long>((d.rows + 31) / 32, std::max<long>(1, 8L * num_sms(d.device) / segments));
+  return static_cast<int>(blocks * segments);
+}
 
 void mx_quantize_launch(const MxQuantDesc& d, cudaStream_t stream) { AVGEN_MX_DISPATCH(quantize, d, stream); }
 void mx_dequantize_launch(const MxDequantDesc& d, cudaStream_t stream) { AVGEN_MX_DISPATCH(dequantize, d, stream); }

@@ -136,6 +136,18 @@ class MXTensor:
         return torch.where(raw == 255, torch.full_like(value, float("nan")), value)
 
 
+def _made(codes: torch.Tensor, scales: torch.Tensor, fmt: str, cols: int, g: torch.Tensor | None) -> MXTensor:
+    """An :class:`MXTensor` of what a kernel returned, without checking it again."""
+    t = object.__new__(MXTensor)
+    put = object.__setattr__
+    put(t, "codes", codes)
+    put(t, "scales", scales)
+    put(t, "fmt", fmt)
+    put(t, "cols", cols)
+    put(t, "global_scale", g)
+    return t
+
+
 def _no_grad_input(what: str, *tensors: torch.Tensor | None) -> None:
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"{what} has no gradient; call it under torch.no_grad() or with detached inputs")
@@ -150,17 +162,16 @@ def quantize(x: torch.Tensor, fmt: str, *, global_scale: torch.Tensor | None = N
     _no_grad_input("quantize", x)
     if global_scale is not None and fid != 2:
         raise ValueError(f"{fmt} has no tensor scale")
-    if x.device.type != "cuda":
+    if not x.is_cuda:
         return _quantize_reference(x, fmt, global_scale)
-    measure = fid == 2 and global_scale is None
-    codes, scales, g = load().mx_quantize(x, fid, global_scale, measure)
-    _count(2 if measure else 1)
-    return MXTensor(codes, scales, fmt, x.shape[-1], g)
+    codes, scales, g, launches = load().mx_quantize(x, fid, global_scale, fid == 2 and global_scale is None)
+    _count(launches)
+    return _made(codes, scales, fmt, x.shape[-1], g)
 
 
 def dequantize(t: MXTensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values ``[rows, cols]`` that ``t`` stands for, in bf16, fp16 or fp32."""
-    if t.device.type != "cuda":
+    if not t.codes.is_cuda:
         return _dequantize_reference(t).to(dtype)
     out = load().mx_dequantize(t.codes, t.scales, _IDS[t.fmt], t.cols, t.global_scale, dtype)
     _count()
@@ -192,13 +203,13 @@ def add_rmsnorm_mod(
     _no_grad_input("add_rmsnorm_mod", x, update, weight, scale, shift, gate)
     if global_scale is not None and fid != 2:
         raise ValueError(f"{fmt} has no tensor scale")
-    if x.device.type != "cuda":
+    if not x.is_cuda:
         return _add_rmsnorm_reference(x, update, weight, scale, shift, gate, rows_per_batch, groups, eps, fmt,
                                       global_scale)
     out, codes, scales = load().mx_add_rmsnorm(x, update, weight, scale, shift, gate, groups, rows_per_batch, eps, fid,
                                                global_scale)
     _count()
-    return out, MXTensor(codes, scales, fmt, x.shape[-1], global_scale)
+    return out, _made(codes, scales, fmt, x.shape[-1], global_scale)
 
 
 def matmul(a: MXTensor, b: MXTensor, *, bias: torch.Tensor | None = None,
@@ -207,8 +218,9 @@ def matmul(a: MXTensor, b: MXTensor, *, bias: torch.Tensor | None = None,
     in fp32 and rounded once to ``out_dtype`` (bf16, fp16 or fp32)."""
     if a.fmt != b.fmt or a.cols != b.cols:
         raise ValueError(f"operands differ: {a.fmt} {a.shape} and {b.fmt} {b.shape}")
-    _no_grad_input("matmul", bias)
-    if a.device.type != "cuda":
+    if bias is not None:
+        _no_grad_input("matmul", bias)
+    if not a.codes.is_cuda:
         out = _dequantize_reference(a) @ _dequantize_reference(b).t()
         return (out if bias is None else out + bias).to(out_dtype)
     out = load().mx_gemm(a.codes, a.scales, a.global_scale, b.codes, b.scales, b.global_scale, _IDS[a.fmt], a.cols,
