@@ -536,11 +536,14 @@ struct Chunk {
       r.pack(v);
       r.load_if(row != nullptr && c < cols, row + c);
     } else {
-      const int end = row != nullptr ? cols : 0;
+      const T* at = row + base + lane;
+      if (row != nullptr && base + kNormSpan <= cols) {  // a whole chunk: no bounds
 #pragma unroll
-      for (int e = 0; e < kNormLane; ++e) {
-        const int c = base + 32 * e + lane;
-        v[e] = c < end ? to_float(row[c]) : other;
+        for (int e = 0; e < kNormLane; ++e) v[e] = to_float(at[32 * e]);
+      } else {
+        const int end = row != nullptr ? cols - base - lane : 0;
+#pragma unroll
+        for (int e = 0; e < kNormLane; ++e) v[e] = 32 * e < end ? to_float(at[32 * e]) : other;
       }
       r.pack(v);
     }
@@ -551,12 +554,17 @@ struct Chunk {
       const int c = base + lane * kNormLane;
       if (c < cols) r.store(row + c);
     } else {
-      float v[kNormLane];
-      r.unpack(v);
+      T* at = row + base + lane;
+      T v[kNormLane];
+      memcpy(v, r.w, sizeof(v));
+      if (base + kNormSpan <= cols) {
 #pragma unroll
-      for (int e = 0; e < kNormLane; ++e) {
-        const int c = base + 32 * e + lane;
-        if (c < cols) row[c] = from_float<T>(v[e]);
+        for (int e = 0; e < kNormLane; ++e) at[32 * e] = v[e];
+      } else {
+        const int end = cols - base - lane;
+#pragma unroll
+        for (int e = 0; e < kNormLane; ++e)
+          if (32 * e < end) at[32 * e] = v[e];
       }
     }
   }
@@ -571,7 +579,8 @@ struct Chunk {
 //
 // The norm takes the fp32 sum x + gate * update, not its rounding to T; statistics,
 // modulation and scaling stay in fp32 until the codes.
-template <typename T, int FMT, int CHUNKS, bool WARP_ROWS, bool ALIGNED>
+// MODULATED = false leaves gate, scale and shift out: their neutral values would cost registers and so CTAs in flight.
+template <typename T, int FMT, int CHUNKS, bool WARP_ROWS, bool ALIGNED, bool MODULATED>
 __global__ void __launch_bounds__(CHUNKS == 8 ? 1024 : 512) mx_add_rmsnorm_kernel(MxNormDesc d, PackedRows p) {
   extern __shared__ __align__(16) float stages[];  // 256 per warp, unaligned rows only
   __shared__ float red[2][32];
@@ -611,13 +620,16 @@ __global__ void __launch_bounds__(CHUNKS == 8 ? 1024 : 512) mx_add_rmsnorm_kerne
 #pragma unroll
     for (int i = 0; i < CHUNKS; ++i) {
       Chunk<float, ALIGNED> t;
-      t.load(gate, base + i * stride, d.W, 1.f);
+      if constexpr (MODULATED) t.load(gate, base + i * stride, d.W, 1.f);
       float u[kNormLane];
       rx[i].r.unpack(v[i]);
       ru[i].r.unpack(u);
 #pragma unroll
       for (int e = 0; e < kNormLane; e += 2) {
-        const Pair x2 = t.pair(e).times_plus(Pair(u[e], u[e + 1]), Pair(v[i][e], v[i][e + 1]));
+        Pair x2(v[i][e], v[i][e + 1]);
+        const Pair u2(u[e], u[e + 1]);
+        if constexpr (MODULATED) x2 = t.pair(e).times_plus(u2, x2);
+        else x2 = x2 + u2;
         x2.get(v[i][e], v[i][e + 1]);
         ss = x2.times_plus(x2, ss);
       }
@@ -647,13 +659,16 @@ __global__ void __launch_bounds__(CHUNKS == 8 ? 1024 : 512) mx_add_rmsnorm_kerne
       const int at = base + i * stride;
       Chunk<float, ALIGNED> w, sc, sh;
       w.load(d.w, at, d.W, 1.f);
-      sc.load(scale, at, d.W);
-      sh.load(shift, at, d.W);
+      if constexpr (MODULATED) {
+        sc.load(scale, at, d.W);
+        sh.load(shift, at, d.W);
+      }
       const Pair r2(r, r), one(1.f, 1.f);
 #pragma unroll
       for (int e = 0; e < kNormLane; e += 2) {
-        const Pair y = Pair(v[i][e], v[i][e + 1]) * r2 * w.pair(e);
-        y.times_plus(sc.pair(e) + one, sh.pair(e)).get(v[i][e], v[i][e + 1]);
+        Pair y = Pair(v[i][e], v[i][e + 1]) * r2 * w.pair(e);
+        if constexpr (MODULATED) y = y.times_plus(sc.pair(e) + one, sh.pair(e));
+        y.get(v[i][e], v[i][e + 1]);
       }
       const int c0 = at + lane * kNormLane;
       if constexpr (!ALIGNED) {
@@ -750,7 +765,9 @@ void dequantize(const MxDequantDesc& d, cudaStream_t stream) {
 
 template <typename T, int FMT, int CHUNKS, bool WARP_ROWS, bool ALIGNED>
 void add_rmsnorm_as(const MxNormDesc& d, const PackedRows& p, int warps, cudaStream_t stream) {
-  auto kernel = mx_add_rmsnorm_kernel<T, FMT, CHUNKS, WARP_ROWS, ALIGNED>;
+  auto kernel = d.gate != nullptr || d.scale != nullptr || d.shift != nullptr
+                    ? mx_add_rmsnorm_kernel<T, FMT, CHUNKS, WARP_ROWS, ALIGNED, true>
+                    : mx_add_rmsnorm_kernel<T, FMT, CHUNKS, WARP_ROWS, ALIGNED, false>;
   const long padded = (d.rows + 127) / 128 * 128;
   const long units = WARP_ROWS ? (padded + warps - 1) / warps : padded;
   const long ctas = static_cast<long>(std::max(1, 64 / warps)) * num_sms(d.device);
