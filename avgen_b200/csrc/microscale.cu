@@ -581,7 +581,7 @@ struct Chunk {
 // modulation and scaling stay in fp32 until the codes.
 // MODULATED = false leaves gate, scale and shift out: their neutral values would cost registers and so CTAs in flight.
 template <typename T, int FMT, int CHUNKS, bool WARP_ROWS, bool ALIGNED, bool MODULATED>
-__global__ void __launch_bounds__(CHUNKS == 8 ? 1024 : 512) mx_add_rmsnorm_kernel(MxNormDesc d, PackedRows p) {
+__global__ void __launch_bounds__(CHUNKS == 8 ? 1024 : 512, CHUNKS <= 2 ? 2 : 1) mx_add_rmsnorm_kernel(MxNormDesc d, PackedRows p) {
   extern __shared__ __align__(16) float stages[];  // 256 per warp, unaligned rows only
   __shared__ float red[2][32];
   const int warp = warp_id(), lane = lane_id();
