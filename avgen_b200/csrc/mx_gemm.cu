@@ -15,6 +15,9 @@
 //               execute in issue order
 //   warps 2..5  epilogue, one TMEM lane quadrant (32 rows) each: TMEM -> registers ->
 //               shared memory -> TMA store, 128 bytes of each row at a time
+// Outputs too small to fill the SMs with such tiles take the split form below it: a
+// cluster of CTAs shares one tile, each with a part of K, and adds up over distributed
+// shared memory in rank order, so results repeat bitwise.
 //
 // In a pair each CTA stages its own 128 rows of A and half of B's 256 rows: the same
 // operand bytes from L2 and shared memory per product as one SM would need for half
@@ -53,7 +56,8 @@ struct Cfg {
   static constexpr int A_BYTES = kBM * kRowBytes;
   static constexpr int B_BYTES = B_ROWS * kRowBytes;
   static constexpr int SFA_BYTES = SF_TILES * 512;
-  static constexpr int SFB_BYTES = BN / 128 * SF_TILES * 512;  // of all BN rows, in both CTAs
+  static constexpr int SFB_GROUPS = (BN + 127) / 128;
+  static constexpr int SFB_BYTES = SFB_GROUPS * SFA_BYTES;  // of all BN rows, in both CTAs
   static constexpr int TX_BYTES = A_BYTES + B_BYTES + SFA_BYTES + SFB_BYTES;
   static constexpr int STAGE_BYTES = (TX_BYTES + 1023) / 1024 * 1024;
   static constexpr int OUT_BYTES = 4 * 2 * kBoxBytes;
@@ -63,7 +67,7 @@ struct Cfg {
   // leave no room for scales, so the second starts inside the first: the epilogue reads
   // the shared columns first and hands them over, and the next tile's products wait for
   // that instead of for a free accumulator.
-  static constexpr int SF_COLS = (SF_TILES * 4 * (1 + BN / 128) + 31) / 32 * 32;
+  static constexpr int SF_COLS = (SF_TILES * 4 * (1 + SFB_GROUPS) + 31) / 32 * 32;
   static constexpr bool OVERLAP = 2 * BN + SF_COLS > 512;
   static constexpr int ACC1 = OVERLAP ? 512 - SF_COLS - BN : BN;
   static constexpr int SF_COL = ACC1 + BN;
@@ -113,12 +117,13 @@ __device__ __forceinline__ void copy_scales(uint32_t taddr, uint32_t smem_addr) 
     asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
 
-// The scales and products of one staged k-block.
+// The scales and products of one staged k-block. `sfb_col`: B's first row within its 128-row
+// scale tile, in columns of 32 rows.
 template <int FMT, int BN, int CTAS>
 __device__ __forceinline__ void issue_block(uint32_t stage_addr, uint32_t tmem_sf, uint32_t tmem_acc, uint32_t idesc,
-                                            int steps, bool first) {
+                                            int steps, bool first, int sfb_col = 0) {
   using C = Cfg<FMT, BN, CTAS>;
-  constexpr int SFB_TILES = (BN + 127) / 128;
+  constexpr int SFB_TILES = C::SFB_GROUPS;
   constexpr int PER = kSteps / C::SF_TILES;  // products per scale tile
   const uint32_t sa = stage_addr, sb = sa + C::A_BYTES, sfa = sb + C::B_BYTES, sfb = sfa + C::SFA_BYTES;
   const uint32_t t_sfb = tmem_sf + C::SF_TILES * 4;
@@ -134,7 +139,7 @@ __device__ __forceinline__ void issue_block(uint32_t stage_addr, uint32_t tmem_s
     if (k < steps) {
       const uint32_t id = static_cast<uint32_t>(k % PER * (4 / PER));  // the step's first scale in its 4-byte cell
       mx_mma<FMT, CTAS>(tmem_acc, umma_desc_sw128(sa + 32 * k, 16, 1024), umma_desc_sw128(sb + 32 * k, 16, 1024),
-                        idesc | (id << 4) | (id << 29), tmem_sf + 4 * (k / PER), t_sfb + (k / PER) * SFB_TILES * 4,
+                        idesc | (id << 4) | (id << 29), tmem_sf + 4 * (k / PER), t_sfb + (k / PER) * SFB_TILES * 4 + sfb_col,
                         (!first || k > 0) ? 1u : 0u);
     }
   }
@@ -448,15 +453,24 @@ __global__ void __launch_bounds__(192, 1)
               store_2d(&tmOut, dst, col, row0);
               bulk_commit_group();
             }
-          } else {  // rows of no 16-byte pitch: lanes along the row
+          } else {  // rows of no 16-byte pitch: a word of the row per lane
             __syncwarp();
-            const int cols = min(BOX, args.N - col);
-            for (int rr = 0; rr < min(32, args.M - row0); ++rr) {
-              T* out = reinterpret_cast<T*>(args.out) + static_cast<long>(row0 + rr) * args.N + col;
-              for (int c = lane; c < cols; c += 32) {
-                const int byte = c * static_cast<int>(sizeof(T));
-                out[c] = *reinterpret_cast<const T*>(dst + rr * 128 + ((byte / 16) ^ (rr & 7)) * 16 + byte % 16);
+            constexpr int PER = 4 / static_cast<int>(sizeof(T));  // values of a word
+            const int c = col + lane * PER;
+            T* out = reinterpret_cast<T*>(args.out) + static_cast<long>(row0) * args.N + c;
+#pragma unroll 8
+            for (int rr = 0; rr < 32; ++rr) {
+              const uint32_t w = *reinterpret_cast<const uint32_t*>(dst + rr * 128 + ((lane / 4) ^ (rr & 7)) * 16 + lane % 4 * 4);
+              if (row0 + rr >= args.M) break;
+              if constexpr (PER == 1) {
+                if (c < args.N) reinterpret_cast<uint32_t*>(out)[0] = w;
+              } else if (args.N % 2 == 0) {
+                if (c < args.N) *reinterpret_cast<uint32_t*>(out) = w;
+              } else {
+                if (c < args.N) reinterpret_cast<uint16_t*>(out)[0] = static_cast<uint16_t>(w);
+                if (c + 1 < args.N) reinterpret_cast<uint16_t*>(out)[1] = static_cast<uint16_t>(w >> 16);
               }
+              out += args.N;
             }
           }
           box ^= 1;
@@ -472,6 +486,159 @@ __global__ void __launch_bounds__(192, 1)
   if (warp == 1) {
     tc_fence_after();
     free_tmem<CTAS>(tmem);
+  }
+}
+
+// ---------------------------------------------------------------- few rows
+// out[m, n] of 128 weight rows (B's, which take the tensor core's 128 lanes) by MT rows
+// of A, over a part of K per CTA of the cluster. What bounds it is the time to stream the
+// weights, so a CTA's whole part is requested at once as far as shared memory goes.
+template <int FMT, int MT>
+struct SplitCfg {
+  using C = Cfg<FMT, MT, 1>;
+  static constexpr int CTAS_PER_SM = MT <= 32 ? 2 : 1;
+  static constexpr int STAGES = std::min(8, (kSmemLimit / CTAS_PER_SM - 2048) / C::STAGE_BYTES);
+  static constexpr int SMEM_BYTES = STAGES * C::STAGE_BYTES + 1024 + 256;
+  static constexpr int TMEM_COLS = MT + C::SF_COLS <= 64 ? 64 : MT + C::SF_COLS <= 128 ? 128 : 256;
+  static_assert(MT * 128 * 4 <= STAGES * C::STAGE_BYTES, "the partial sums reuse the ring");
+};
+
+template <typename T, int FMT, int MT>
+__global__ void __launch_bounds__(192, 1)
+    mx_gemm_split_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
+                         const __grid_constant__ CUtensorMap tmSFW, const __grid_constant__ CUtensorMap tmSFX,
+                         const int splits, const int kb_per_split, const MxArgs args) {
+  using S = SplitCfg<FMT, MT>;
+  using C = typename S::C;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::STAGES * C::STAGE_BYTES);
+  uint64_t* empty = full + S::STAGES;
+  uint64_t* tfull = empty + S::STAGES;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tfull + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = warp_id();
+  const int lane = lane_id();
+  const int rank = blockIdx.x % splits;  // clusters lie along x
+  const int n0 = blockIdx.x / splits * 128, m0 = blockIdx.y * MT;
+  const int kb0 = rank * kb_per_split, kb1 = min(args.num_kb, kb0 + kb_per_split);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S::STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(tfull, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, S::TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      for (int kb = kb0, i = 0; kb < kb1; ++kb, ++i) {
+        const int stage = i % S::STAGES;
+        if (i >= S::STAGES &&
+            !mbar_wait(&empty[stage], (i / S::STAGES - 1) & 1, abort_flag, args.err, kErrTimeoutProducer)) {
+          let_copies_land();
+          break;
+        }
+        uint8_t* sw = smem + stage * C::STAGE_BYTES;
+        uint8_t* sx = sw + C::A_BYTES;
+        uint8_t* sfw = sx + C::B_BYTES;
+        mbar_arrive_expect_tx(&full[stage], C::TX_BYTES);
+        const uint32_t bar = smem_u32(&full[stage]);
+        load_2d<1>(sw, &tmW, bar, kb * kRowBytes, n0);
+        load_2d<1>(sx, &tmX, bar, kb * kRowBytes, m0);
+        load_3d<1>(sfw, &tmSFW, bar, 0, kb * C::SF_TILES, n0 / 128);
+        load_3d<1>(sfw + C::SFA_BYTES, &tmSFX, bar, 0, kb * C::SF_TILES, m0 / 128);
+      }
+    }
+  } else if (warp == 1) {
+    constexpr uint32_t idesc = mx_idesc<FMT>(128, MT);
+    bool aborted = false;
+    for (int kb = kb0, i = 0; kb < kb1; ++kb, ++i) {
+      const int stage = i % S::STAGES;
+      if (!mbar_wait(&full[stage], (i / S::STAGES) & 1, abort_flag, args.err, kErrTimeoutMma)) {
+        aborted = true;
+        break;
+      }
+      tc_fence_after();
+      if (elect_one()) {
+        issue_block<FMT, MT, 1>(smem_u32(smem + stage * C::STAGE_BYTES), tmem + MT, tmem, idesc,
+                                kb == args.num_kb - 1 ? args.last_steps : kSteps, kb == kb0, m0 % 128 / 32);
+        mma_commit(&empty[stage]);
+      }
+      __syncwarp();
+    }
+    if (!aborted && elect_one()) mma_commit(tfull);
+    __syncwarp();
+  } else if (mbar_wait(tfull, 0, abort_flag, args.err, kErrTimeoutEpilogue)) {
+    tc_fence_after();
+    const int q = warp & 3;
+    const int lane_n = q * 32 + lane, n = n0 + lane_n;
+    const int rows = min(MT, args.M - m0);
+    const float alpha = (args.a_g != nullptr ? *args.a_g : 1.f) * (args.b_g != nullptr ? *args.b_g : 1.f);
+    const float bias = args.bias != nullptr && n < args.N ? args.bias[n] : 0.f;
+    float* partial = reinterpret_cast<float*>(smem);  // [row][128 weight rows]: every staged block has been multiplied
+#pragma unroll
+    for (int c = 0; c < MT / 32; ++c) {
+      if (32 * c >= rows) break;
+      uint32_t r[32];
+      tmem_ld32(tmem + (static_cast<uint32_t>(q * 32) << 16) + 32 * c, r);
+      tmem_wait_ld();
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        const int m = 32 * c + i;
+        if (m >= rows) break;
+        if (splits > 1)
+          partial[m * 128 + lane_n] = __uint_as_float(r[i]);
+        else if (n < args.N)
+          reinterpret_cast<T*>(args.out)[static_cast<long>(m0 + m) * args.N + n] =
+              from_float<T>(fmaf(__uint_as_float(r[i]), alpha, bias));
+      }
+    }
+  }
+  tc_fence_before();
+  if (splits > 1) {
+    cluster_sync();
+    if (warp >= 2) {
+      const int lane_n = (warp & 3) * 32 + lane, n = n0 + lane_n;
+      const int rows = min(MT, args.M - m0);
+      const float alpha = (args.a_g != nullptr ? *args.a_g : 1.f) * (args.b_g != nullptr ? *args.b_g : 1.f);
+      const float bias = args.bias != nullptr && n < args.N ? args.bias[n] : 0.f;
+      const uint32_t mine = smem_u32(smem) + static_cast<uint32_t>(lane_n) * 4u;
+      for (int m = rank; m < rows; m += splits) {
+        float part[8];
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+          part[s] = 0.f;
+          if (s < splits)
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(part[s]) : "r"(map_to_rank(mine, s) + m * 512u) : "memory");
+        }
+        float sum = part[0];
+#pragma unroll
+        for (int s = 1; s < 8; ++s)
+          if (s < splits) sum += part[s];
+        if (n < args.N)
+          reinterpret_cast<T*>(args.out)[static_cast<long>(m0 + m) * args.N + n] = from_float<T>(fmaf(sum, alpha, bias));
+      }
+    }
+    cluster_sync();  // no CTA leaves while another reads its sums
+  } else {
+    __syncthreads();
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, S::TMEM_COLS);
   }
 }
 
@@ -542,6 +709,34 @@ void launch_tiles(const MxGemmDesc& d, const MxArgs& args, cudaStream_t stream) 
   AVGEN_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, ta, tb, tsa, tsb, to, tma_out, args));
 }
 
+template <typename T, int FMT, int MT>
+void launch_split(const MxGemmDesc& d, const MxArgs& args, int splits, cudaStream_t stream) {
+  using S = SplitCfg<FMT, MT>;
+  using C = typename S::C;
+  const long row_bytes = mx_row_bytes(FMT, d.K), tiles_k = mx_scale_tiles(FMT, d.K);
+  const CUtensorMap tw = codes_map(d.b_codes, row_bytes, d.N, 128);
+  const CUtensorMap tx = codes_map(d.a_codes, row_bytes, d.M, MT);
+  const CUtensorMap tsw = scales_map(d.b_scales, tiles_k, d.N, C::SF_TILES, 1);
+  const CUtensorMap tsx = scales_map(d.a_scales, tiles_k, d.M, C::SF_TILES, 1);
+  auto kernel = mx_gemm_split_kernel<T, FMT, MT>;
+  static PerDeviceOnce once;
+  raise_smem_limit(once, kernel, S::SMEM_BYTES);
+  const int per = (args.num_kb + splits - 1) / splits;
+  splits = (args.num_kb + per - 1) / per;  // every CTA has a part
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>((d.N + 127) / 128 * splits), static_cast<unsigned>((d.M + MT - 1) / MT));
+  cfg.blockDim = dim3(192);
+  cfg.dynamicSmemBytes = S::SMEM_BYTES;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = static_cast<unsigned>(splits);
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = splits > 1 ? 1 : 0;
+  AVGEN_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, tw, tx, tsw, tsx, splits, per, args));
+}
+
 template <typename T, int FMT>
 void launch(const MxGemmDesc& d, cudaStream_t stream) {
   MxArgs args{};
@@ -551,8 +746,20 @@ void launch(const MxGemmDesc& d, cudaStream_t stream) {
   args.last_steps = static_cast<int>((row_bytes - static_cast<long>(args.num_kb - 1) * kRowBytes + 31) / 32);
   args.a_g = d.a_g, args.b_g = d.b_g;
   args.bias = d.bias, args.out = d.out, args.err = d.err;
-  const long pair_tiles = static_cast<long>((d.M + 255) / 256) * ((d.N + 255) / 256);
-  if (pair_tiles * 2 >= num_sms(d.device)) return launch_tiles<T, FMT, 256, 2>(d, args, stream);
+  // A k-block costs a CTA about as much in every form: its operand bytes from L2 (32 to 38
+  // KB at some 45 bytes a clock). So the form with the fewest rounds of k-blocks wins: split
+  // ones take 1 / splits of a round, 256 x 256 tiles one round for every SMs / 2 of them,
+  // 128 x 128 tiles one for every SMs.
+  const int sms = num_sms(d.device);
+  const long tiles = static_cast<long>((d.M + 127) / 128) * ((d.N + 127) / 128);
+  const long pairs = static_cast<long>((d.M + 255) / 256) * ((d.N + 255) / 256);
+  if (d.M <= 32) {
+    const long room = SplitCfg<FMT, 32>::CTAS_PER_SM * sms / tiles;
+    return launch_split<T, FMT, 32>(d, args, static_cast<int>(std::clamp<long>(room, 1, std::min(8, args.num_kb))), stream);
+  }
+  if (2 * tiles <= sms && args.num_kb > 1)
+    return launch_split<T, FMT, 128>(d, args, static_cast<int>(std::min<long>({8, sms / tiles, args.num_kb})), stream);
+  if ((pairs + sms / 2 - 1) / (sms / 2) <= (tiles + sms - 1) / sms) return launch_tiles<T, FMT, 256, 2>(d, args, stream);
   launch_tiles<T, FMT, 128, 1>(d, args, stream);
 }
 
