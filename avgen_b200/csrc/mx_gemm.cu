@@ -104,48 +104,64 @@ __device__ __forceinline__ void mx_mma(uint32_t d, uint64_t a, uint64_t b, uint3
 #undef AVGEN_MX_MMA
 }
 
-// One scale tile (512 bytes of shared memory: 32 rows of 16 bytes) to four TMEM
-// columns, repeated in all four lane quadrants; in a pair, in each CTA from its own
-// shared memory.
+// A scale tile in shared memory: 32 rows of 16 bytes, no swizzle, 8-row groups 128 bytes apart.
+__device__ __forceinline__ uint64_t scale_desc(uint32_t smem_addr) {
+  return static_cast<uint64_t>((smem_addr >> 4) & 0x3FFFu) | (static_cast<uint64_t>(128 >> 4) << 32) | (1ull << 46);
+}
+// One scale tile to four TMEM columns, repeated in all four lane quadrants; in a pair, in
+// each CTA from its own shared memory.
 template <int CTAS>
-__device__ __forceinline__ void copy_scales(uint32_t taddr, uint32_t smem_addr) {
-  const uint64_t desc = static_cast<uint64_t>((smem_addr >> 4) & 0x3FFFu) | (static_cast<uint64_t>(128 >> 4) << 32) |
-                        (1ull << 46);  // no swizzle, 8-row groups 128 bytes apart
+__device__ __forceinline__ void copy_scales(uint32_t taddr, uint64_t desc) {
   if constexpr (CTAS == 1)
     asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
   else
     asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
 
-// The scales and products of one staged k-block. `sfb_col`: B's first row within its 128-row
-// scale tile, in columns of 32 rows.
+// Descriptors of stage 0 and the tensor-memory places, from which a stage's follow by one
+// addition (addresses are below 2^18 bytes, so the 14-bit field does not carry).
 template <int FMT, int BN, int CTAS>
-__device__ __forceinline__ void issue_block(uint32_t stage_addr, uint32_t tmem_sf, uint32_t tmem_acc, uint32_t idesc,
-                                            int steps, bool first, int sfb_col = 0) {
+struct Issuer {
   using C = Cfg<FMT, BN, CTAS>;
-  constexpr int SFB_TILES = C::SFB_GROUPS;
-  constexpr int PER = kSteps / C::SF_TILES;  // products per scale tile
-  const uint32_t sa = stage_addr, sb = sa + C::A_BYTES, sfa = sb + C::B_BYTES, sfb = sfa + C::SFA_BYTES;
-  const uint32_t t_sfb = tmem_sf + C::SF_TILES * 4;
-#pragma unroll
-  for (int i = 0; i < C::SF_TILES; ++i) {
-    copy_scales<CTAS>(tmem_sf + 4 * i, sfa + 512 * i);
-#pragma unroll
-    for (int j = 0; j < SFB_TILES; ++j)
-      copy_scales<CTAS>(t_sfb + (i * SFB_TILES + j) * 4, sfb + j * C::SFA_BYTES + 512 * i);
+  static constexpr int SFB_TILES = C::SFB_GROUPS;
+  static constexpr int PER = kSteps / C::SF_TILES;  // products per scale tile
+  uint64_t a, b, sfa, sfb;
+  uint32_t t_sfa, t_sfb;
+
+  // `sf`: TMEM address of the scales.
+  __device__ __forceinline__ Issuer(uint32_t smem_addr, uint32_t sf) {
+    a = umma_desc_sw128(smem_addr, 16, 1024);
+    b = umma_desc_sw128(smem_addr + C::A_BYTES, 16, 1024);
+    sfa = scale_desc(smem_addr + C::A_BYTES + C::B_BYTES);
+    sfb = scale_desc(smem_addr + C::A_BYTES + C::B_BYTES + C::SFA_BYTES);
+    t_sfa = sf;
+    t_sfb = sf + C::SF_TILES * 4;
   }
+  // The scales and products of one staged k-block.
+  __device__ __forceinline__ void block(int stage, uint32_t tmem_acc, uint32_t idesc, int steps, bool first) const {
+    const uint32_t at = static_cast<uint32_t>(stage) * (C::STAGE_BYTES / 16);
 #pragma unroll
-  for (int k = 0; k < kSteps; ++k) {
-    if (k < steps) {
-      const uint32_t id = static_cast<uint32_t>(k % PER * (4 / PER));  // the step's first scale in its 4-byte cell
-      mx_mma<FMT, CTAS>(tmem_acc, umma_desc_sw128(sa + 32 * k, 16, 1024), umma_desc_sw128(sb + 32 * k, 16, 1024),
-                        idesc | (id << 4) | (id << 29), tmem_sf + 4 * (k / PER), t_sfb + (k / PER) * SFB_TILES * 4 + sfb_col,
-                        (!first || k > 0) ? 1u : 0u);
+    for (int i = 0; i < C::SF_TILES; ++i) {
+      copy_scales<CTAS>(t_sfa + 4 * i, sfa + at + 32 * i);
+#pragma unroll
+      for (int j = 0; j < SFB_TILES; ++j)
+        copy_scales<CTAS>(t_sfb + (i * SFB_TILES + j) * 4, sfb + at + j * (C::SFA_BYTES / 16) + 32 * i);
+    }
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) {
+      if (k < steps) {
+        const uint32_t id = static_cast<uint32_t>(k % PER * (4 / PER));  // the step's first scale in its 4-byte cell
+        mx_mma<FMT, CTAS>(tmem_acc, a + at + 2 * k, b + at + 2 * k, idesc | (id << 4) | (id << 29),
+                          t_sfa + 4 * (k / PER), t_sfb + (k / PER) * SFB_TILES * 4, (!first || k > 0) ? 1u : 0u);
+      }
     }
   }
-}
+};
 
 // ---------------------------------------------------------------- pair plumbing
+// The warp's number as a value the compiler knows to be uniform.
+__device__ __forceinline__ int uniform_warp_id() { return __shfl_sync(0xffffffffu, warp_id(), 0); }
+
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -298,7 +314,7 @@ __global__ void __launch_bounds__(192, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int warp = warp_id();
+  const int warp = uniform_warp_id();
   const int lane = lane_id();
   const int rank = CTAS == 2 ? static_cast<int>(cluster_rank()) : 0;
   const int num_m = (args.M + CTAS * kBM - 1) / (CTAS * kBM);
@@ -332,40 +348,46 @@ __global__ void __launch_bounds__(192, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
+  // Both issuing roles run warp-uniform with one elected thread: from a divergent branch
+  // each TMA or tcgen05 instruction takes several times as long to issue (mxfp8 32768 x
+  // 5120 x 5120: products issued by `if (lane == 0)` ran at 2.2 instead of 2.8 PFLOP/s).
   if (warp == 0) {
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      bool aborted = false;
-      for (int t = first; t < num_tiles && !aborted; t += step) {
-        int tm, tn;
-        tile_at(t, num_m, num_n, tm, tn);
-        for (int kb = 0; kb < args.num_kb; ++kb) {
-          if (!mbar_wait(&empty[stage], phase ^ 1, abort_flag, args.err, kErrTimeoutProducer)) {
-            aborted = true;
-            break;
-          }
+    int stage = 0;
+    uint32_t phase = 0;
+    bool aborted = false;
+    const uint32_t bar0 = CTAS == 2 ? map_to_rank(smem_u32(full), 0) : smem_u32(full);
+    for (int t = first; t < num_tiles && !aborted; t += step) {
+      int tm, tn;
+      tile_at(t, num_m, num_n, tm, tn);
+      for (int kb = 0; kb < args.num_kb; ++kb) {
+        if (!mbar_wait(&empty[stage], phase ^ 1, abort_flag, args.err, kErrTimeoutProducer)) {
+          aborted = true;
+          break;
+        }
+        if (elect_one()) {
           uint8_t* sa = smem + stage * C::STAGE_BYTES;
           uint8_t* sb = sa + C::A_BYTES;
           uint8_t* sfa = sb + C::B_BYTES;
           uint8_t* sfb = sfa + C::SFA_BYTES;
           if (rank == 0) mbar_arrive_expect_tx(&full[stage], CTAS * C::TX_BYTES);
-          const uint32_t bar = CTAS == 2 ? map_to_rank(smem_u32(&full[stage]), 0) : smem_u32(&full[stage]);
+          const uint32_t bar = bar0 + stage * 8;
           load_2d<CTAS>(sa, &tmA, bar, kb * kRowBytes, (tm * CTAS + rank) * kBM);
           load_2d<CTAS>(sb, &tmB, bar, kb * kRowBytes, tn * BN + rank * C::B_ROWS);
           load_3d<CTAS>(sfa, &tmSFA, bar, 0, kb * C::SF_TILES, tm * CTAS + rank);
           load_3d<CTAS>(sfb, &tmSFB, bar, 0, kb * C::SF_TILES, tn * (BN / 128));
-          if (++stage == C::STAGES) {
-            stage = 0;
-            phase ^= 1;
-          }
+        }
+        __syncwarp();
+        if (++stage == C::STAGES) {
+          stage = 0;
+          phase ^= 1;
         }
       }
-      if (aborted) let_copies_land();
     }
+    if (aborted) let_copies_land();
   } else if (warp == 1) {
     if (rank == 0) {
       constexpr uint32_t idesc = mx_idesc<FMT>(CTAS * kBM, BN);
+      const Issuer<FMT, BN, CTAS> issue(smem_u32(smem), tmem + C::SF_COL);
       int stage = 0;
       uint32_t phase = 0;
       bool aborted = false;
@@ -383,8 +405,7 @@ __global__ void __launch_bounds__(192, 1)
           }
           tc_fence_after();
           if (elect_one()) {
-            issue_block<FMT, BN, CTAS>(smem_u32(smem + stage * C::STAGE_BYTES), tmem + C::SF_COL, tmem + acc * C::ACC1,
-                                       idesc, kb == args.num_kb - 1 ? args.last_steps : kSteps, kb == 0);
+            issue.block(stage, tmem + acc * C::ACC1, idesc, kb == args.num_kb - 1 ? args.last_steps : kSteps, kb == 0);
             commit<CTAS>(&empty[stage]);
           }
           __syncwarp();
@@ -493,6 +514,8 @@ __global__ void __launch_bounds__(192, 1)
 // out[m, n] of 128 weight rows (B's, which take the tensor core's 128 lanes) by MT rows
 // of A, over a part of K per CTA of the cluster. What bounds it is the time to stream the
 // weights, so a CTA's whole part is requested at once as far as shared memory goes.
+constexpr int kMaxSplits = 8;  // CTAs of a portable cluster
+
 template <int FMT, int MT>
 struct SplitCfg {
   using C = Cfg<FMT, MT, 1>;
@@ -518,7 +541,7 @@ __global__ void __launch_bounds__(192, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tfull + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int warp = warp_id();
+  const int warp = uniform_warp_id();
   const int lane = lane_id();
   const int rank = blockIdx.x % splits;  // clusters lie along x
   const int n0 = blockIdx.x / splits * 128, m0 = blockIdx.y * MT;
@@ -543,14 +566,14 @@ __global__ void __launch_bounds__(192, 1)
   const uint32_t tmem = *tmem_slot;
 
   if (warp == 0) {
-    if (lane == 0) {
-      for (int kb = kb0, i = 0; kb < kb1; ++kb, ++i) {
-        const int stage = i % S::STAGES;
-        if (i >= S::STAGES &&
-            !mbar_wait(&empty[stage], (i / S::STAGES - 1) & 1, abort_flag, args.err, kErrTimeoutProducer)) {
-          let_copies_land();
-          break;
-        }
+    for (int kb = kb0, i = 0; kb < kb1; ++kb, ++i) {
+      const int stage = i % S::STAGES;
+      if (i >= S::STAGES &&
+          !mbar_wait(&empty[stage], (i / S::STAGES - 1) & 1, abort_flag, args.err, kErrTimeoutProducer)) {
+        let_copies_land();
+        break;
+      }
+      if (elect_one()) {
         uint8_t* sw = smem + stage * C::STAGE_BYTES;
         uint8_t* sx = sw + C::A_BYTES;
         uint8_t* sfw = sx + C::B_BYTES;
@@ -561,9 +584,11 @@ __global__ void __launch_bounds__(192, 1)
         load_3d<1>(sfw, &tmSFW, bar, 0, kb * C::SF_TILES, n0 / 128);
         load_3d<1>(sfw + C::SFA_BYTES, &tmSFX, bar, 0, kb * C::SF_TILES, m0 / 128);
       }
+      __syncwarp();
     }
   } else if (warp == 1) {
     constexpr uint32_t idesc = mx_idesc<FMT>(128, MT);
+    const Issuer<FMT, MT, 1> issue(smem_u32(smem), tmem + MT);
     bool aborted = false;
     for (int kb = kb0, i = 0; kb < kb1; ++kb, ++i) {
       const int stage = i % S::STAGES;
@@ -573,8 +598,7 @@ __global__ void __launch_bounds__(192, 1)
       }
       tc_fence_after();
       if (elect_one()) {
-        issue_block<FMT, MT, 1>(smem_u32(smem + stage * C::STAGE_BYTES), tmem + MT, tmem, idesc,
-                                kb == args.num_kb - 1 ? args.last_steps : kSteps, kb == kb0, m0 % 128 / 32);
+        issue.block(stage, tmem, idesc, kb == args.num_kb - 1 ? args.last_steps : kSteps, kb == kb0);
         mma_commit(&empty[stage]);
       }
       __syncwarp();
@@ -610,26 +634,37 @@ __global__ void __launch_bounds__(192, 1)
   tc_fence_before();
   if (splits > 1) {
     cluster_sync();
-    if (warp >= 2) {
-      const int lane_n = (warp & 3) * 32 + lane, n = n0 + lane_n;
+    if (warp >= 2) {  // a warp per row, four columns per lane, every CTA's part requested before the first is added
+      const int n = n0 + 4 * lane;
       const int rows = min(MT, args.M - m0);
       const float alpha = (args.a_g != nullptr ? *args.a_g : 1.f) * (args.b_g != nullptr ? *args.b_g : 1.f);
-      const float bias = args.bias != nullptr && n < args.N ? args.bias[n] : 0.f;
-      const uint32_t mine = smem_u32(smem) + static_cast<uint32_t>(lane_n) * 4u;
-      for (int m = rank; m < rows; m += splits) {
-        float part[8];
+      float bias[4];
 #pragma unroll
-        for (int s = 0; s < 8; ++s) {
-          part[s] = 0.f;
+      for (int j = 0; j < 4; ++j) bias[j] = args.bias != nullptr && n + j < args.N ? args.bias[n + j] : 0.f;
+      uint32_t part_at[kMaxSplits];
+#pragma unroll
+      for (int s = 0; s < kMaxSplits; ++s) part_at[s] = map_to_rank(smem_u32(smem) + lane * 16u, min(s, splits - 1));
+#pragma unroll 2
+      for (int m = rank + splits * (warp & 3); m < rows; m += 4 * splits) {
+        float4 part[kMaxSplits];
+#pragma unroll
+        for (int s = 0; s < kMaxSplits; ++s) {
+          part[s] = make_float4(0.f, 0.f, 0.f, 0.f);
           if (s < splits)
-            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(part[s]) : "r"(map_to_rank(mine, s) + m * 512u) : "memory");
+            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                         : "=f"(part[s].x), "=f"(part[s].y), "=f"(part[s].z), "=f"(part[s].w)
+                         : "r"(part_at[s] + m * 512u)
+                         : "memory");
         }
-        float sum = part[0];
+        float4 sum = part[0];
 #pragma unroll
-        for (int s = 1; s < 8; ++s)
-          if (s < splits) sum += part[s];
-        if (n < args.N)
-          reinterpret_cast<T*>(args.out)[static_cast<long>(m0 + m) * args.N + n] = from_float<T>(fmaf(sum, alpha, bias));
+        for (int s = 1; s < kMaxSplits; ++s)
+          sum.x += part[s].x, sum.y += part[s].y, sum.z += part[s].z, sum.w += part[s].w;
+        const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+        T* out = reinterpret_cast<T*>(args.out) + static_cast<long>(m0 + m) * args.N + n;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (n + j < args.N) out[j] = from_float<T>(fmaf(v[j], alpha, bias[j]));
       }
     }
     cluster_sync();  // no CTA leaves while another reads its sums
@@ -755,10 +790,10 @@ void launch(const MxGemmDesc& d, cudaStream_t stream) {
   const long pairs = static_cast<long>((d.M + 255) / 256) * ((d.N + 255) / 256);
   if (d.M <= 32) {
     const long room = SplitCfg<FMT, 32>::CTAS_PER_SM * sms / tiles;
-    return launch_split<T, FMT, 32>(d, args, static_cast<int>(std::clamp<long>(room, 1, std::min(8, args.num_kb))), stream);
+    return launch_split<T, FMT, 32>(d, args, static_cast<int>(std::clamp<long>(room, 1, std::min(kMaxSplits, args.num_kb))), stream);
   }
   if (2 * tiles <= sms && args.num_kb > 1)
-    return launch_split<T, FMT, 128>(d, args, static_cast<int>(std::min<long>({8, sms / tiles, args.num_kb})), stream);
+    return launch_split<T, FMT, 128>(d, args, static_cast<int>(std::min<long>({kMaxSplits, sms / tiles, args.num_kb})), stream);
   if ((pairs + sms / 2 - 1) / (sms / 2) <= (tiles + sms - 1) / sms) return launch_tiles<T, FMT, 256, 2>(d, args, stream);
   launch_tiles<T, FMT, 128, 1>(d, args, stream);
 }
