@@ -36,6 +36,8 @@ def add_parser(subparsers: Any) -> None:
     s.add_argument("--guidance-rescale", type=float, default=None)
     s.add_argument("--sampler", default="", choices=("", "euler", "heun", "dpmpp_2m", "res_multistep"))
     s.add_argument("--seed", type=int, default=-1)
+    s.add_argument("--quantize", default="", choices=("", "mxfp8", "mxfp4", "nvfp4"),
+                   help="run the DiT blocks' linears on 8- or 4-bit block-scaled weights and activations")
     geo = p.add_argument_group("output geometry (latent units)")
     geo.add_argument("--frames", type=int, default=0)
     geo.add_argument("--height", type=int, default=0)
@@ -103,6 +105,10 @@ def run(args: argparse.Namespace) -> int:
     model = build_model(config)
     _load_weights(Path(args.checkpoint), model)
     model.to(device).eval()
+    if args.quantize:
+        from avgen_b200.models import quantize_model
+
+        quantize_model(model, args.quantize)
     video, text = _codecs(args, config)
     pipe = GenerationPipeline(model, video_codec=video, text_encoder=text, config=settings, device=device)
     bsz = args.batch_size or inf.batch_size

@@ -4,6 +4,7 @@ from avgen_b200.models.blocks import CrossModalFusion, DiTBlock, RopeInputs, Tex
 from avgen_b200.models.dit import AVDiT, AVDiTConfig, VideoDiT, VideoDiTConfig, list_presets, preset
 from avgen_b200.models.layers import (AdaLNModulation, CrossAttention, FusedRMSNorm, GeluMLP, SelfAttention, SwiGLU,
                                       TimestepEmbedding, modulate, sinusoidal_embedding)
+from avgen_b200.models.quantized import quantize_model, restore_model
 from avgen_b200.models.registry import build_model, list_models, model_config_class, register_model
 from avgen_b200.models.rope import RoPEScaling, RotaryEmbedding, RotaryTables, apply_rotary, build_rotary_tables
 
@@ -12,7 +13,8 @@ __all__ = [
     "GeluMLP", "RoPEScaling", "RopeInputs", "RotaryEmbedding", "RotaryTables", "SelfAttention", "SwiGLU",
     "TextRefinerBlock", "TimestepEmbedding", "VideoDiT", "VideoDiTConfig", "apply_rotary", "attention",
     "build_model", "build_rotary_tables", "device_arch", "key_padding_mask", "list_models", "list_presets",
-    "model_config_class", "modulate", "preset", "register_model", "sinusoidal_embedding", "temporal_neighbour_mask",
+    "model_config_class", "modulate", "preset", "quantize_model", "register_model",
+    "restore_model", "sinusoidal_embedding", "temporal_neighbour_mask",
 ]
 
 # constants and helpers the reference also exports at this level

@@ -116,6 +116,7 @@ class DiTBlock(nn.Module):
         self.scale_shift_table = nn.Parameter(torch.zeros(MODULATION_CHUNKS, width))
         self.attention_impl = None  # set by context parallelism for the fused path
         self.use_fused = True
+        self.quantized = None  # packed weights set by quantize_model: the block runs on them, without a gradient
 
     def forward(self, hidden: torch.Tensor, *, modulation: torch.Tensor, rope: RotaryTables | RopeInputs | None = None,
                 key_mask: torch.Tensor | None = None, context: torch.Tensor | None = None,
@@ -130,6 +131,11 @@ class DiTBlock(nn.Module):
         if modulation_index is not None and modulation.ndim != 3:
             raise ValueError("modulation_index selects rows of a (rows, 6, width) modulation")
         combined = modulation + self.scale_shift_table
+        if self.quantized is not None:
+            from avgen_b200.models.quantized import quantized_block_forward
+
+            return quantized_block_forward(self, hidden, combined, rope=rope, key_mask=key_mask, context=context,
+                                           context_mask=context_mask, mod_index=modulation_index)
         if (self.use_fused and _fused_eligible(self, hidden)
                 and (rope is None or isinstance(rope, RopeInputs))):
             return self._fused(hidden, combined, rope, key_mask, context, context_mask, modulation_index)

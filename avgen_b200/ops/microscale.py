@@ -149,8 +149,10 @@ def _made(codes: torch.Tensor, scales: torch.Tensor, fmt: str, cols: int, g: tor
 
 
 def _no_grad_input(what: str, *tensors: torch.Tensor | None) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{what} has no gradient; call it under torch.no_grad() or with detached inputs")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{what} has no gradient; call it under torch.no_grad() or with detached inputs")
 
 
 def quantize(x: torch.Tensor, fmt: str, *, global_scale: torch.Tensor | None = None) -> MXTensor:

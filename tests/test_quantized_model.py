@@ -1,0 +1,185 @@
+"""Quantised DiT blocks: against the same block with each linear's operands rounded to the
+format, and against the unquantised block; what quantising refuses and leaves alone."""
+from __future__ import annotations
+
+import copy
+
+import pytest
+import torch
+from torch import nn
+
+import microscale_oracle as oracle
+from avgen_b200.models import DiTBlock, RopeInputs, RotaryEmbedding, quantize_model, restore_model
+from avgen_b200.ops import microscale as mx
+
+# The error a format may add to a block's output, relative to its norm. An element is off by
+# at most half a spacing: a relative 2^-4 in e4m3 (rms about 2^-4 / sqrt(3) = 0.036 / 2) and
+# 2^-2 in e2m1 (rms 0.14 / 2); seven products in a row, each with two rounded operands whose
+# errors add as squares, and a residual stream that carries most of the output.
+BOUND = {"mxfp8": 0.036 / 2 * 14 ** 0.5, "mxfp4": 0.14 * 14 ** 0.5 / 2, "nvfp4": 0.14 * 14 ** 0.5 / 2}
+
+
+def _block(width: int = 256, heads: int = 2, **more: object) -> DiTBlock:
+    block = DiTBlock(width, heads, hidden=2 * width, **more)
+    block.init_weights(depth=2)
+    with torch.no_grad():
+        for p in block.parameters():
+            p.add_(0.02 * torch.randn_like(p))
+    return block
+
+
+def _inputs(form: str, device: str = "cpu", dtype: torch.dtype = torch.float32) -> tuple[torch.Tensor, dict]:
+    b, length, width = 2, 160, 256
+    rope = RopeInputs((torch.rand(b, length, 3) * 8).to(device), RotaryEmbedding(128))
+    index = None
+    if form == "grouped":
+        mod = 0.1 * torch.randn(2 * b, 6, width)
+        index = (torch.arange(b)[:, None] * 2 + (torch.arange(length) < 40).long()[None]).int().to(device)
+    elif form == "token":
+        mod = 0.1 * torch.randn(b, length, 6, width)
+    else:
+        mod = 0.1 * torch.randn(b, 6, width)
+    key = torch.ones(b, length, dtype=torch.bool)
+    key[0, 120:] = False
+    text = torch.ones(b, 24, dtype=torch.bool)
+    text[1, 20:] = False
+    kwargs = {"modulation": mod.to(device), "rope": rope, "key_mask": key.to(device), "modulation_index": index,
+              "context": torch.randn(b, 24, width).to(device, dtype), "context_mask": text.to(device)}
+    return torch.randn(b, length, width).to(device, dtype), kwargs
+
+
+def _rounded_block(block: DiTBlock, fmt: str, monkeypatch: pytest.MonkeyPatch) -> None:
+    """Every linear of the eager block multiplies rounded operands (mxfp8 and mxfp4: no tensor scale to share)."""
+    from avgen_b200.models import layers
+
+    def rounded(x: torch.Tensor, layer: nn.Linear) -> torch.Tensor:
+        w = mx.dequantize(mx.quantize(layer.weight.detach(), fmt), torch.float32)
+        xq = mx.dequantize(mx.quantize(x.reshape(-1, x.shape[-1]), fmt), torch.float32)
+        return (xq @ w.t()).view(*x.shape[:-1], -1)
+
+    monkeypatch.setattr(layers, "linear", rounded)
+
+
+@pytest.mark.parametrize("fmt", ["mxfp8", "mxfp4"])
+@pytest.mark.parametrize("ffn,form", [("swiglu", "sample"), ("gelu", "grouped"), ("swiglu", "token")])
+def test_block_is_the_eager_block_on_rounded_operands(fmt: str, ffn: str, form: str,
+                                                      monkeypatch: pytest.MonkeyPatch) -> None:
+    torch.manual_seed(0)
+    block = _block(ffn=ffn)
+    hidden, kwargs = _inputs(form)
+    with torch.no_grad():
+        assert quantize_model(block, fmt) == 1
+        got = block(hidden, **kwargs)
+        restore_model(block)
+        _rounded_block(block, fmt, monkeypatch)
+        want = block(hidden, **kwargs)
+    # the same rounding at every linear; fp32 sums in another order move single elements across
+    # a rounding boundary, a spacing each, in few places
+    assert float((got - want).norm() / want.norm()) < 2e-3
+
+
+@pytest.mark.parametrize("fmt", mx.FORMATS)
+def test_block_stays_near_the_unquantised_block(fmt: str) -> None:
+    torch.manual_seed(1)
+    block = _block()
+    hidden, kwargs = _inputs("grouped")
+    with torch.no_grad():
+        want = block(hidden, **kwargs)
+        quantize_model(block, fmt)
+        got = block(hidden, **kwargs)
+        assert 0 < float((got - want).norm() / want.norm()) < BOUND[fmt]
+        assert restore_model(block) == 1 and restore_model(block) == 0
+        assert torch.equal(block(hidden, **kwargs), want)
+
+
+def test_without_cross_attention_and_with_adapters() -> None:
+    from avgen_b200.finetune import LoRAConfig, apply_lora
+
+    torch.manual_seed(2)
+    block = _block(cross_attention=False)
+    hidden, kwargs = _inputs("sample")
+    kwargs["context"] = None
+    with torch.no_grad():
+        quantize_model(block, "mxfp8")
+        block(hidden, **kwargs)
+    apply_lora(block, LoRAConfig(rank=4, target_modules=("q_proj", "up_proj")))
+    with torch.no_grad():
+        for name, p in block.named_parameters():
+            if name.endswith("lora_b"):
+                p.normal_(std=0.1)
+        restore_model(block)
+        want = block(hidden, **kwargs)
+        quantize_model(block, "mxfp8")
+        assert float((block(hidden, **kwargs) - want).norm() / want.norm()) < BOUND["mxfp8"]
+
+
+def test_state_and_refusals() -> None:
+    block = _block()
+    keys = set(block.state_dict())
+    hidden, kwargs = _inputs("sample")
+    quantize_model(block, "nvfp4")
+    assert set(block.state_dict()) == keys
+    packed = block.quantized
+    plain = sum(p.numel() for n, p in block.named_parameters() if "proj" in n)
+    assert plain * 9 / 16 <= packed.nbytes <= plain * 9 / 16 * 1.01
+    with pytest.raises(RuntimeError, match="no gradient"):
+        block(hidden, **kwargs)
+    assert copy.deepcopy(block).quantized.fmt == "nvfp4"
+    with pytest.raises(ValueError, match="format must be"):
+        quantize_model(block, "int4")
+    other = _block()
+    other.attention_impl = object()
+    with pytest.raises(ValueError, match="context parallelism"):
+        quantize_model(other, "mxfp8")
+    biased = _block()
+    biased.attention.q_proj = nn.Linear(256, 256)
+    with pytest.raises(ValueError, match="no bias"):
+        quantize_model(nn.ModuleList([_block(), biased]), "mxfp8")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", mx.FORMATS)
+@pytest.mark.parametrize("ffn,form", [("swiglu", "sample"), ("gelu", "grouped"), ("swiglu", "token")])
+def test_gpu_block_stays_near_the_fp32_block(fmt: str, ffn: str, form: str) -> None:
+    from avgen_b200.ops._ext import check_errors
+
+    torch.manual_seed(3)
+    block = _block(ffn=ffn)
+    hidden, kwargs = _inputs(form)
+    with torch.no_grad():
+        want = block(hidden, **kwargs)
+        block.cuda()
+        quantize_model(block, fmt)
+        kwargs = {k: v.cuda() if isinstance(v, torch.Tensor) else v for k, v in kwargs.items()}
+        kwargs["rope"] = RopeInputs(kwargs["rope"].coords.cuda(), kwargs["rope"].rope)
+        kwargs["context"] = kwargs["context"].bfloat16()
+        got = block(hidden.cuda().bfloat16(), **kwargs)
+    assert got.dtype is torch.bfloat16
+    assert float((got.float().cpu() - want).norm() / want.norm()) < BOUND[fmt] + 2e-2  # the bf16 residual stream
+    assert check_errors() == 0
+
+
+@pytest.mark.gpu
+def test_gpu_model_samples_quantised() -> None:
+    from dataclasses import asdict
+
+    from avgen_b200.codecs import ReferenceTextEncoder, ReferenceVideoCodec
+    from avgen_b200.infer import GenerationConfig, GenerationPipeline, ScheduleConfig
+    from avgen_b200.models import build_model, preset
+
+    torch.manual_seed(4)
+    cfg = {k: v for k, v in asdict(preset("tiny_gpu")).items() if k != "rope_scaling"}
+    model = build_model("video_dit", cfg).cuda().eval()
+    model.init_weights()
+    with torch.no_grad():
+        for p in model.parameters():
+            p.add_(0.02 * torch.randn_like(p))
+    video = ReferenceVideoCodec(channels=cfg["in_channels"], temporal_compression=1, spatial_compression=1)
+    text = ReferenceTextEncoder(width=cfg["text_width"], max_length=16)
+    settings = GenerationConfig(steps=2, height=32, width=32, num_frames=4, schedule=ScheduleConfig(steps=2))
+    pipe = GenerationPipeline(model, video_codec=video, text_encoder=text, config=settings, device=torch.device("cuda"))
+    full = pipe(["a kite"], seed=1).video.float()
+    assert quantize_model(model, "mxfp8") == cfg["depth"]
+    packed = pipe(["a kite"], seed=1).video.float()
+    assert torch.isfinite(packed).all()
+    assert float((packed - full).norm() / full.norm()) < 0.2
