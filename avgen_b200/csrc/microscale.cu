@@ -819,8 +819,8 @@ void add_rmsnorm(const MxNormDesc& d, cudaStream_t stream) {
 int mx_quantize_parts(const MxQuantDesc& d) {
   const long segments = segments_of(d.cols);
   if (d.rows * segments <= kSmallWarps * kSmallCtas) return 0;
-  // CTAs of the measuring pass: up to eight for every SM, 32 rows of 512 columns at least
-  const long blocks = std::min<long>((d.rows + 31) / 32, std::max<long>(1, 8L * num_sms(d.device) / segments));
+  // CTAs of the measuring pass: up to eight for every SM, a row per warp at least
+  const long blocks = std::min<long>((d.rows + 7) / 8, std::max<long>(1, 8L * num_sms(d.device) / segments));
   return static_cast<int>(blocks * segments);
 }
 

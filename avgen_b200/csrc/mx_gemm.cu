@@ -13,8 +13,8 @@
 //   warp 1      MMA issuer (the pair's first CTA): copies a stage's scales to TMEM
 //               (tcgen05.cp), then issues its products; both kinds of instruction
 //               execute in issue order
-//   warps 2..5  epilogue, one TMEM lane quadrant (32 rows) each: TMEM -> registers ->
-//               shared memory -> TMA store, 128 bytes of each row at a time
+//   warps 2..9  epilogue, two per TMEM lane quadrant (32 rows), half the columns each:
+//               TMEM -> registers -> shared memory -> TMA store, 128 bytes of a row at a time
 // Outputs too small to fill the SMs with such tiles take the split form below it: a
 // cluster of CTAs shares one tile, each with a part of K, and adds up over distributed
 // shared memory in rank order, so results repeat bitwise.
@@ -48,6 +48,10 @@ constexpr int kRowBytes = 128;  // code bytes of a row in one k-block: one swizz
 constexpr int kSteps = 4;       // products per k-block, 32 code bytes each
 constexpr int kBoxBytes = 32 * 128;  // one warp's store: 32 rows x 128 bytes
 constexpr int kSmemLimit = 232448;
+// Two epilogue warps per quadrant: with one, a 256 x 256 tile took 4.6 us to store, longer
+// than the products of K = 2560 in 4 bits.
+constexpr int kEpiWarps = 8;
+constexpr int kThreads = 64 + 32 * kEpiWarps;
 
 template <int FMT, int BN, int CTAS>
 struct Cfg {
@@ -60,7 +64,7 @@ struct Cfg {
   static constexpr int SFB_BYTES = SFB_GROUPS * SFA_BYTES;  // of all BN rows, in both CTAs
   static constexpr int TX_BYTES = A_BYTES + B_BYTES + SFA_BYTES + SFB_BYTES;
   static constexpr int STAGE_BYTES = (TX_BYTES + 1023) / 1024 * 1024;
-  static constexpr int OUT_BYTES = 4 * 2 * kBoxBytes;
+  static constexpr int OUT_BYTES = kEpiWarps * kBoxBytes;
   static constexpr int STAGES = std::min(8, (kSmemLimit - 2048 - OUT_BYTES) / STAGE_BYTES);
   static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + OUT_BYTES + 1024 + 256;
   // TMEM: two accumulators and the scales of one k-block. Two 256-column accumulators
@@ -298,8 +302,35 @@ __device__ __forceinline__ void stage_row(uint8_t* box, int lane, const float* v
   }
 }
 
+// A staged box to rows of no 16-byte pitch: a word of the row per lane, eight rows in flight.
+template <typename T>
+__device__ __forceinline__ void store_box_words(const MxArgs& args, const uint8_t* box, int lane, int row0, int col) {
+  constexpr int WORD = 4 / static_cast<int>(sizeof(T));  // values of a word
+  const int c = col + lane * WORD;
+  const bool first = c < args.N, second = c + 1 < args.N, words = WORD == 1 || args.N % 2 == 0;
+  T* out = reinterpret_cast<T*>(args.out) + static_cast<long>(row0) * args.N + c;
+  for (int r0 = 0; r0 < min(32, args.M - row0); r0 += 8) {
+    uint32_t w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      w[i] = *reinterpret_cast<const uint32_t*>(box + (r0 + i) * 128 + ((lane / 4) ^ i) * 16 + lane % 4 * 4);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (row0 + r0 + i < args.M) {
+        if (words) {
+          if (first) *reinterpret_cast<uint32_t*>(out) = w[i];
+        } else {
+          if (first) reinterpret_cast<uint16_t*>(out)[0] = static_cast<uint16_t>(w[i]);
+          if (second) reinterpret_cast<uint16_t*>(out)[1] = static_cast<uint16_t>(w[i] >> 16);
+        }
+      }
+      out += args.N;
+    }
+  }
+}
+
 template <typename T, int FMT, int BN, int CTAS>
-__global__ void __launch_bounds__(192, 1)
+__global__ void __launch_bounds__(kThreads, 1)
     mx_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                    const __grid_constant__ CUtensorMap tmSFA, const __grid_constant__ CUtensorMap tmSFB,
                    const __grid_constant__ CUtensorMap tmOut, const bool tma_out, const MxArgs args) {
@@ -329,7 +360,7 @@ __global__ void __launch_bounds__(192, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&tfull[b], 1);
-      mbar_init(&tempty[b], 4 * CTAS);
+      mbar_init(&tempty[b], kEpiWarps * CTAS);
     }
     *abort_flag = 0;
     fence_barrier_init();
@@ -420,33 +451,42 @@ __global__ void __launch_bounds__(192, 1)
       }
     }
   } else {
-    constexpr int GROUPS = BN / 64;                  // of 64 columns
+    constexpr int GROUPS = BN / 64 / 2;                     // groups of 64 columns of this warp's half
     constexpr int BOX = 128 / static_cast<int>(sizeof(T));  // columns of a store box
-    const int q = warp & 3;
-    uint8_t* boxes = smem_out + (warp - 2) * 2 * kBoxBytes;
+    const int q = warp & 3, half = (warp - 2) >> 2;
+    uint8_t* box = smem_out + (warp - 2) * kBoxBytes;
     const float alpha = (args.a_g != nullptr ? *args.a_g : 1.f) * (args.b_g != nullptr ? *args.b_g : 1.f);
     uint32_t release[2];
     for (int b = 0; b < 2; ++b)
       release[b] = CTAS == 2 ? map_to_rank(smem_u32(&tempty[b]), 0) : smem_u32(&tempty[b]);
-    int i = 0, box = 0;
+    int i = 0;
     for (int t = first; t < num_tiles; t += step, ++i) {
       int tm, tn;
       tile_at(t, num_m, num_n, tm, tn);
       const int acc = i & 1;
       if (!mbar_wait(&tfull[acc], (i >> 1) & 1, abort_flag, args.err, kErrTimeoutEpilogue)) break;
       tc_fence_after();
+      // What this warp has to have read before the next tile's products may start: with
+      // overlapping accumulators the shared columns (the first one's last, the second one's
+      // first group) if they are in its half, else nothing of this tile (its arrival says
+      // that it is done with the tile before); without overlap all of its half.
+      const bool holds_shared = C::OVERLAP && half == 1 - acc;
+      if (C::OVERLAP && !holds_shared) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive_at(release[acc]);
+      }
       const int row0 = (tm * CTAS + rank) * kBM + q * 32;
 #pragma unroll
       for (int step_g = 0; step_g < GROUPS; ++step_g) {
-        // the columns shared with the next accumulator first: the first accumulator's last ones
-        const int g = C::OVERLAP && acc == 0 ? GROUPS - 1 - step_g : step_g;
+        const int g = half * GROUPS + (C::OVERLAP && acc == 0 ? GROUPS - 1 - step_g : step_g);  // shared columns first
         uint32_t r[2][32];
         const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16) + acc * C::ACC1 + 64 * g;
         tmem_ld32(taddr, r[0]);
         tmem_ld32(taddr + 32, r[1]);
         tmem_wait_ld();
-        if (step_g == (C::OVERLAP ? 0 : GROUPS - 1)) {
-          static_assert(!C::OVERLAP || BN - C::ACC1 <= 64, "shared columns lie in one group");
+        static_assert(!C::OVERLAP || BN - C::ACC1 <= 64, "shared columns lie in one group");
+        if (C::OVERLAP ? holds_shared && step_g == 0 : step_g == GROUPS - 1) {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) arrive_at(release[acc]);
@@ -463,38 +503,20 @@ __global__ void __launch_bounds__(192, 1)
 #pragma unroll
         for (int h = 0; h < 64 / BOX; ++h) {
           const int col = col0 + BOX * h;
-          uint8_t* dst = boxes + box * kBoxBytes;
-          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+          if (lane == 0) bulk_wait_group_read0();
           __syncwarp();
-          stage_row<T>(dst, lane, v + BOX * h);
+          stage_row<T>(box, lane, v + BOX * h);
           if (tma_out) {
             fence_proxy_async();
             __syncwarp();
             if (lane == 0 && col < args.N) {
-              store_2d(&tmOut, dst, col, row0);
+              store_2d(&tmOut, box, col, row0);
               bulk_commit_group();
             }
-          } else {  // rows of no 16-byte pitch: a word of the row per lane
+          } else {
             __syncwarp();
-            constexpr int PER = 4 / static_cast<int>(sizeof(T));  // values of a word
-            const int c = col + lane * PER;
-            T* out = reinterpret_cast<T*>(args.out) + static_cast<long>(row0) * args.N + c;
-#pragma unroll 8
-            for (int rr = 0; rr < 32; ++rr) {
-              const uint32_t w = *reinterpret_cast<const uint32_t*>(dst + rr * 128 + ((lane / 4) ^ (rr & 7)) * 16 + lane % 4 * 4);
-              if (row0 + rr >= args.M) break;
-              if constexpr (PER == 1) {
-                if (c < args.N) reinterpret_cast<uint32_t*>(out)[0] = w;
-              } else if (args.N % 2 == 0) {
-                if (c < args.N) *reinterpret_cast<uint32_t*>(out) = w;
-              } else {
-                if (c < args.N) reinterpret_cast<uint16_t*>(out)[0] = static_cast<uint16_t>(w);
-                if (c + 1 < args.N) reinterpret_cast<uint16_t*>(out)[1] = static_cast<uint16_t>(w >> 16);
-              }
-              out += args.N;
-            }
+            store_box_words<T>(args, box, lane, row0, col);
           }
-          box ^= 1;
         }
       }
     }
@@ -641,6 +663,7 @@ __global__ void __launch_bounds__(192, 1)
       float bias[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) bias[j] = args.bias != nullptr && n + j < args.N ? args.bias[n + j] : 0.f;
+      const bool whole = args.N % 4 == 0 && n < args.N;
       uint32_t part_at[kMaxSplits];
 #pragma unroll
       for (int s = 0; s < kMaxSplits; ++s) part_at[s] = map_to_rank(smem_u32(smem) + lane * 16u, min(s, splits - 1));
@@ -660,11 +683,17 @@ __global__ void __launch_bounds__(192, 1)
 #pragma unroll
         for (int s = 1; s < kMaxSplits; ++s)
           sum.x += part[s].x, sum.y += part[s].y, sum.z += part[s].z, sum.w += part[s].w;
-        const float v[4] = {sum.x, sum.y, sum.z, sum.w};
         T* out = reinterpret_cast<T*>(args.out) + static_cast<long>(m0 + m) * args.N + n;
+        alignas(16) T v[4] = {from_float<T>(fmaf(sum.x, alpha, bias[0])), from_float<T>(fmaf(sum.y, alpha, bias[1])),
+                              from_float<T>(fmaf(sum.z, alpha, bias[2])), from_float<T>(fmaf(sum.w, alpha, bias[3]))};
+        if (whole) {  // rows on 4 values
+          if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(v);
+          else *reinterpret_cast<uint4*>(out) = *reinterpret_cast<const uint4*>(v);
+        } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (n + j < args.N) out[j] = from_float<T>(fmaf(v[j], alpha, bias[j]));
+          for (int j = 0; j < 4; ++j)
+            if (n + j < args.N) out[j] = v[j];
+        }
       }
     }
     cluster_sync();  // no CTA leaves while another reads its sums
@@ -732,7 +761,7 @@ void launch_tiles(const MxGemmDesc& d, const MxArgs& args, cudaStream_t stream) 
   AVGEN_CHECK(tiles < (1L << 30), "mx_gemm: too many output tiles");
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(CTAS * std::min<long>(tiles, num_sms(d.device) / CTAS)));
-  cfg.blockDim = dim3(192);
+  cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = C::SMEM_BYTES;
   cfg.stream = stream;
   cudaLaunchAttribute attr{};
@@ -744,8 +773,28 @@ void launch_tiles(const MxGemmDesc& d, const MxArgs& args, cudaStream_t stream) 
   AVGEN_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, ta, tb, tsa, tsb, to, tma_out, args));
 }
 
+// Clusters of 1..kMaxSplits CTAs that the device holds at once: a cluster stays within one
+// GPC, so larger ones leave SMs idle.
+struct ClusterRoom {
+  int clusters[kMaxSplits + 1] = {};
+};
+
+// Fewest rounds of k-blocks, a round and its setup counted as kSplitSetup of them.
+constexpr int kSplitSetup = 8;
+
+inline int choose_splits(const ClusterRoom& room, long tiles, int num_kb) {
+  int best = 1;
+  long cost = 0;
+  for (int s = 1; s <= std::min(kMaxSplits, num_kb); ++s) {
+    if (room.clusters[s] < 1) continue;
+    const long c = (tiles + room.clusters[s] - 1) / room.clusters[s] * ((num_kb + s - 1) / s + kSplitSetup);
+    if (s == 1 || c < cost) best = s, cost = c;
+  }
+  return best;
+}
+
 template <typename T, int FMT, int MT>
-void launch_split(const MxGemmDesc& d, const MxArgs& args, int splits, cudaStream_t stream) {
+void launch_split(const MxGemmDesc& d, const MxArgs& args, cudaStream_t stream) {
   using S = SplitCfg<FMT, MT>;
   using C = typename S::C;
   const long row_bytes = mx_row_bytes(FMT, d.K), tiles_k = mx_scale_tiles(FMT, d.K);
@@ -754,21 +803,32 @@ void launch_split(const MxGemmDesc& d, const MxArgs& args, int splits, cudaStrea
   const CUtensorMap tsw = scales_map(d.b_scales, tiles_k, d.N, C::SF_TILES, 1);
   const CUtensorMap tsx = scales_map(d.a_scales, tiles_k, d.M, C::SF_TILES, 1);
   auto kernel = mx_gemm_split_kernel<T, FMT, MT>;
-  static PerDeviceOnce once;
+  static PerDeviceOnce once, asked;
   raise_smem_limit(once, kernel, S::SMEM_BYTES);
-  const int per = (args.num_kb + splits - 1) / splits;
-  splits = (args.num_kb + per - 1) / per;  // every CTA has a part
+  const unsigned tiles_n = static_cast<unsigned>((d.N + 127) / 128), tiles_m = static_cast<unsigned>((d.M + MT - 1) / MT);
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>((d.N + 127) / 128 * splits), static_cast<unsigned>((d.M + MT - 1) / MT));
   cfg.blockDim = dim3(192);
   cfg.dynamicSmemBytes = S::SMEM_BYTES;
   cfg.stream = stream;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = static_cast<unsigned>(splits);
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
-  cfg.numAttrs = splits > 1 ? 1 : 0;
+  cfg.numAttrs = 1;
+  static ClusterRoom rooms[kMaxDevices];
+  ClusterRoom& room = rooms[d.device];
+  asked.run(d.device, [&] {
+    for (int s = 1; s <= kMaxSplits; ++s) {
+      cfg.gridDim = dim3(static_cast<unsigned>(s));
+      attr.val.clusterDim.x = static_cast<unsigned>(s);
+      AVGEN_CUDA_CHECK(cudaOccupancyMaxActiveClusters(&room.clusters[s], kernel, &cfg));
+    }
+  });
+  int splits = choose_splits(room, static_cast<long>(tiles_n) * tiles_m, args.num_kb);
+  const int per = (args.num_kb + splits - 1) / splits;
+  splits = (args.num_kb + per - 1) / per;  // every CTA has a part
+  cfg.gridDim = dim3(tiles_n * splits, tiles_m);
+  attr.val.clusterDim.x = static_cast<unsigned>(splits);
   AVGEN_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, tw, tx, tsw, tsx, splits, per, args));
 }
 
@@ -788,12 +848,8 @@ void launch(const MxGemmDesc& d, cudaStream_t stream) {
   const int sms = num_sms(d.device);
   const long tiles = static_cast<long>((d.M + 127) / 128) * ((d.N + 127) / 128);
   const long pairs = static_cast<long>((d.M + 255) / 256) * ((d.N + 255) / 256);
-  if (d.M <= 32) {
-    const long room = SplitCfg<FMT, 32>::CTAS_PER_SM * sms / tiles;
-    return launch_split<T, FMT, 32>(d, args, static_cast<int>(std::clamp<long>(room, 1, std::min(kMaxSplits, args.num_kb))), stream);
-  }
-  if (2 * tiles <= sms && args.num_kb > 1)
-    return launch_split<T, FMT, 128>(d, args, static_cast<int>(std::min<long>({kMaxSplits, sms / tiles, args.num_kb})), stream);
+  if (d.M <= 32) return launch_split<T, FMT, 32>(d, args, stream);
+  if (2 * tiles <= sms && args.num_kb > 1) return launch_split<T, FMT, 128>(d, args, stream);
   if ((pairs + sms / 2 - 1) / (sms / 2) <= (tiles + sms - 1) / sms) return launch_tiles<T, FMT, 256, 2>(d, args, stream);
   launch_tiles<T, FMT, 128, 1>(d, args, stream);
 }
