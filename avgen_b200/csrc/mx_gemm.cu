@@ -773,24 +773,20 @@ void launch_tiles(const MxGemmDesc& d, const MxArgs& args, cudaStream_t stream) 
   AVGEN_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, ta, tb, tsa, tsb, to, tma_out, args));
 }
 
-// Clusters of 1..kMaxSplits CTAs that the device holds at once: a cluster stays within one
-// GPC, so larger ones leave SMs idle.
+// Clusters of 1..kMaxSplits CTAs, a CTA per SM, that the device holds at once: a cluster
+// stays within one GPC, so larger ones leave SMs idle (148, 74, 45, 33, 26, 22, 15, 15).
 struct ClusterRoom {
   int clusters[kMaxSplits + 1] = {};
 };
 
-// Fewest rounds of k-blocks, a round and its setup counted as kSplitSetup of them.
-constexpr int kSplitSetup = 8;
-
+// As many parts as leave every tile its cluster at once. More would put two CTAs on some
+// SMs, which then share what an SM takes in (1 x 15360 x 2560 nvfp4, 120 tiles: one part 5.8
+// us, two 7.3), or wait for a second round (77 x 2560 x 4096 mxfp8, 20 tiles: six parts 7.5
+// us, seven 13).
 inline int choose_splits(const ClusterRoom& room, long tiles, int num_kb) {
-  int best = 1;
-  long cost = 0;
-  for (int s = 1; s <= std::min(kMaxSplits, num_kb); ++s) {
-    if (room.clusters[s] < 1) continue;
-    const long c = (tiles + room.clusters[s] - 1) / room.clusters[s] * ((num_kb + s - 1) / s + kSplitSetup);
-    if (s == 1 || c < cost) best = s, cost = c;
-  }
-  return best;
+  int s = std::min(kMaxSplits, num_kb);
+  while (s > 1 && room.clusters[s] < tiles) --s;
+  return s;
 }
 
 template <typename T, int FMT, int MT>
