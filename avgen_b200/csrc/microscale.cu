@@ -26,18 +26,8 @@ __device__ __forceinline__ void load32(const void* p, uint32_t* w) {
       : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
       : "l"(p));
 }
-// As load32 where `on`, else the words keep what they hold: a load without a branch.
-__device__ __forceinline__ void load32_if(bool on, const void* p, uint32_t* w) {
-  asm("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %9, 0;\n\t"
-      "@q ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n\t}"
-      : "+r"(w[0]), "+r"(w[1]), "+r"(w[2]), "+r"(w[3]), "+r"(w[4]), "+r"(w[5]), "+r"(w[6]), "+r"(w[7])
-      : "l"(p), "r"(static_cast<int>(on)));
-}
-__device__ __forceinline__ void load16_if(bool on, const void* p, uint32_t* w) {
-  asm("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-      "@q ld.global.nc.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}"
-      : "+r"(w[0]), "+r"(w[1]), "+r"(w[2]), "+r"(w[3])
-      : "l"(p), "r"(static_cast<int>(on)));
+__device__ __forceinline__ void load16(const void* p, uint32_t* w) {
+  asm("ld.global.nc.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(p));
 }
 __device__ __forceinline__ void store32(void* p, const uint32_t* w) {
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
@@ -120,16 +110,11 @@ struct Raw {
 
   // From / to an address on 32 bytes (or on all of a shorter run).
   __device__ __forceinline__ void load(const T* p) {
-    static_assert(WORDS % 8 == 0, "whole 32-byte loads");
-#pragma unroll
-    for (int i = 0; i < WORDS; i += 8) load32(reinterpret_cast<const uint32_t*>(p) + i, w + i);
-  }
-  __device__ __forceinline__ void load_if(bool on, const T* p) {
     if constexpr (WORDS == 4) {
-      load16_if(on, p, w);
+      load16(p, w);
     } else {
 #pragma unroll
-      for (int i = 0; i < WORDS; i += 8) load32_if(on, reinterpret_cast<const uint32_t*>(p) + i, w + i);
+      for (int i = 0; i < WORDS; i += 8) load32(reinterpret_cast<const uint32_t*>(p) + i, w + i);
     }
   }
   __device__ __forceinline__ void store(T* p) const {
@@ -519,31 +504,47 @@ __global__ void __launch_bounds__(256) mx_dequantize_kernel(MxDequantDesc d, Pac
 constexpr int kNormLane = 8;  // columns of a lane in one chunk: fp32 modulation rows in 32-byte loads side by side
 constexpr int kNormSpan = 32 * kNormLane;
 
+// What a missing row reads as, in the aligned layout (eight columns, the same for every lane).
+__device__ const __align__(32) float kNormZeros[kNormLane] = {};
+__device__ const __align__(32) float kNormOnes[kNormLane] = {1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f};
+
+// A row of the input or of a modulation, or `other` (0 or 1) in every column where there
+// is none. An aligned row is read without conditions: lanes past its end read its first
+// columns, a missing row is a short constant one.
+template <typename T, bool ALIGNED>
+struct NormRow {
+  const T* row;
+  int mask;  // of a lane's column
+  float other;
+
+  __device__ __forceinline__ NormRow(const T* base, long at, float other_) : other(other_) {
+    mask = base != nullptr ? ~0 : 0;
+    row = base != nullptr ? base + at : nullptr;
+    if (ALIGNED && base == nullptr) row = reinterpret_cast<const T*>(other_ == 0.f ? kNormZeros : kNormOnes);
+  }
+};
+
 // Eight columns per lane of the 256-column chunk at `base`: consecutive ones of an
 // aligned row, every 32nd of any other.
 template <typename T, bool ALIGNED>
 struct Chunk {
   Raw<T, kNormLane> r;
 
-  // `other` past the row's end, and everywhere when there is no such row.
-  __device__ __forceinline__ void load(const T* row, int base, int cols, float other = 0.f) {
-    const int lane = lane_id();
-    float v[kNormLane];
+  // `column`: the lane's first one in this chunk, or 0 where that lies past the row's end.
+  __device__ __forceinline__ void load(const NormRow<T, ALIGNED>& from, int base, int column, int cols) {
     if constexpr (ALIGNED) {
-      const int c = base + lane * kNormLane;
-#pragma unroll
-      for (int e = 0; e < kNormLane; ++e) v[e] = other;
-      r.pack(v);
-      r.load_if(row != nullptr && c < cols, row + c);
+      r.load(from.row + (column & from.mask));
     } else {
-      const T* at = row + base + lane;
-      if (row != nullptr && base + kNormSpan <= cols) {  // a whole chunk: no bounds
+      const int lane = lane_id();
+      const T* at = from.row + base + lane;
+      float v[kNormLane];
+      if (from.row != nullptr && base + kNormSpan <= cols) {  // a whole chunk: no bounds
 #pragma unroll
         for (int e = 0; e < kNormLane; ++e) v[e] = to_float(at[32 * e]);
       } else {
-        const int end = row != nullptr ? cols - base - lane : 0;
+        const int end = from.row != nullptr ? cols - base - lane : 0;
 #pragma unroll
-        for (int e = 0; e < kNormLane; ++e) v[e] = 32 * e < end ? to_float(at[32 * e]) : other;
+        for (int e = 0; e < kNormLane; ++e) v[e] = 32 * e < end ? to_float(at[32 * e]) : from.other;
       }
       r.pack(v);
     }
@@ -594,36 +595,42 @@ __global__ void __launch_bounds__(CHUNKS == 8 ? 1024 : 512, CHUNKS <= 2 ? 2 : 1)
   int row = WARP_ROWS ? blockIdx.x * (blockDim.x >> 5) + warp : blockIdx.x;
   const int base = place * kNormSpan, stride = warps * kNormSpan;  // of the warp's chunks
 
-  // A missing update, gate, weight, scale or shift reads as 0, 1, 1, 0 and 0: no branches, so loads are issued together.
+  int column[CHUNKS];  // of the lane's first value in each chunk, 0 past the end
+#pragma unroll
+  for (int i = 0; i < CHUNKS; ++i) {
+    const int c = base + i * stride + lane * kNormLane;
+    column[i] = c < d.W ? c : 0;
+  }
   Chunk<T, ALIGNED> rx[CHUNKS], ru[CHUNKS];
   int next_b = 0;
   auto request = [&](int at) {
     if (d.num_groups > 0) next_b = static_cast<int>(mod_row(d.groups, d.num_groups, at, d.rows_per_batch));
-    const T* x = reinterpret_cast<const T*>(d.x) + at * d.ldx;
-    const T* u = d.update != nullptr ? reinterpret_cast<const T*>(d.update) + at * d.ldu : nullptr;
+    const NormRow<T, ALIGNED> x(reinterpret_cast<const T*>(d.x), at * d.ldx, 0.f);
+    const NormRow<T, ALIGNED> u(reinterpret_cast<const T*>(d.update), at * d.ldu, 0.f);
 #pragma unroll
     for (int i = 0; i < CHUNKS; ++i) {
-      rx[i].load(x, base + i * stride, d.W);
-      ru[i].load(u, base + i * stride, d.W);
+      rx[i].load(x, base + i * stride, column[i], d.W);
+      ru[i].load(u, base + i * stride, column[i], d.W);
     }
   };
-  auto level = [](const float* t, long at) { return t != nullptr ? t + at : nullptr; };
+  const NormRow<float, ALIGNED> weight(d.w, 0, 1.f);
   if (row < rows) request(row);
   int turn = 0;
   for (; row < rows; row += step) {
     float v[CHUNKS][kNormLane];
-    const float* gate = level(d.gate, next_b * d.gate_stride);
-    const float* scale = level(d.scale, next_b * d.mod_stride);
-    const float* shift = level(d.shift, next_b * d.mod_stride);
+    const NormRow<float, ALIGNED> gate(d.gate, next_b * d.gate_stride, 1.f);
+    const NormRow<float, ALIGNED> scale(d.scale, next_b * d.mod_stride, 0.f);
+    const NormRow<float, ALIGNED> shift(d.shift, next_b * d.mod_stride, 0.f);
     T* x_out = reinterpret_cast<T*>(d.x_out) + static_cast<long>(row) * d.W;
     Pair ss(0.f, 0.f);
 #pragma unroll
     for (int i = 0; i < CHUNKS; ++i) {
       Chunk<float, ALIGNED> t;
-      if constexpr (MODULATED) t.load(gate, base + i * stride, d.W, 1.f);
+      if constexpr (MODULATED) t.load(gate, base + i * stride, column[i], d.W);
       float u[kNormLane];
       rx[i].r.unpack(v[i]);
       ru[i].r.unpack(u);
+      const bool past = ALIGNED && base + i * stride + lane * kNormLane >= d.W;
 #pragma unroll
       for (int e = 0; e < kNormLane; e += 2) {
         Pair x2(v[i][e], v[i][e + 1]);
@@ -631,6 +638,14 @@ __global__ void __launch_bounds__(CHUNKS == 8 ? 1024 : 512, CHUNKS <= 2 ? 2 : 1)
         if constexpr (MODULATED) x2 = t.pair(e).times_plus(u2, x2);
         else x2 = x2 + u2;
         x2.get(v[i][e], v[i][e + 1]);
+      }
+      if (past) {
+#pragma unroll
+        for (int e = 0; e < kNormLane; ++e) v[i][e] = 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < kNormLane; e += 2) {
+        const Pair x2(v[i][e], v[i][e + 1]);
         ss = x2.times_plus(x2, ss);
       }
       if (d.x_out != nullptr) {
@@ -658,10 +673,10 @@ __global__ void __launch_bounds__(CHUNKS == 8 ? 1024 : 512, CHUNKS <= 2 ? 2 : 1)
     for (int i = 0; i < CHUNKS; ++i) {
       const int at = base + i * stride;
       Chunk<float, ALIGNED> w, sc, sh;
-      w.load(d.w, at, d.W, 1.f);
+      w.load(weight, at, column[i], d.W);
       if constexpr (MODULATED) {
-        sc.load(scale, at, d.W);
-        sh.load(shift, at, d.W);
+        sc.load(scale, at, column[i], d.W);
+        sh.load(shift, at, column[i], d.W);
       }
       const Pair r2(r, r), one(1.f, 1.f);
 #pragma unroll

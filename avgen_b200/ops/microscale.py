@@ -70,9 +70,9 @@ def _scale_bytes(fmt: str, rows: int, cols: int) -> int:
     return -(-rows // 128) * -(-cols // (4 * block_size(fmt))) * 512
 
 
-@dataclass(frozen=True, slots=True, eq=False)
+@dataclass(slots=True, eq=False)
 class MXTensor:
-    """A packed matrix ``[rows, cols]``.
+    """A packed matrix ``[rows, cols]``. Its fields are set once, here or by the operators.
 
     ``codes`` is uint8 ``[rows, bytes]``: one row's codes, columns padded with zero
     codes to a multiple of 32; 4-bit codes two to a byte, the even column in the low
@@ -138,13 +138,8 @@ class MXTensor:
 
 def _made(codes: torch.Tensor, scales: torch.Tensor, fmt: str, cols: int, g: torch.Tensor | None) -> MXTensor:
     """An :class:`MXTensor` of what a kernel returned, without checking it again."""
-    t = object.__new__(MXTensor)
-    put = object.__setattr__
-    put(t, "codes", codes)
-    put(t, "scales", scales)
-    put(t, "fmt", fmt)
-    put(t, "cols", cols)
-    put(t, "global_scale", g)
+    t = MXTensor.__new__(MXTensor)
+    t.codes, t.scales, t.fmt, t.cols, t.global_scale = codes, scales, fmt, cols, g
     return t
 
 
@@ -161,7 +156,8 @@ def quantize(x: torch.Tensor, fmt: str, *, global_scale: torch.Tensor | None = N
     ``global_scale`` (nvfp4): a positive fp32 ``[1]`` tensor scale to use, e.g. a
     calibrated one; without it one pass over ``x`` measures it first."""
     fid = _format_id(fmt)
-    _no_grad_input("quantize", x)
+    if x.requires_grad:
+        _no_grad_input("quantize", x)
     if global_scale is not None and fid != 2:
         raise ValueError(f"{fmt} has no tensor scale")
     if not x.is_cuda:
