@@ -337,7 +337,7 @@ __global__ void __launch_bounds__(256) mx_amax_kernel(MxQuantDesc d) {
 
 // A CTA quantises `rows_per_cta` rows x 512 columns, a warp one row at a time.
 template <typename T, int FMT, bool ALIGNED>
-__global__ void __launch_bounds__(256) mx_quantize_kernel(MxQuantDesc d, PackedRows p, int rows_per_cta) {
+__global__ void __launch_bounds__(256, ALIGNED ? 4 : 2) mx_quantize_kernel(MxQuantDesc d, PackedRows p, int rows_per_cta) {
   constexpr int UNROLL = ALIGNED && sizeof(T) == 2 ? 4 : 2;
   __shared__ __align__(16) T stage[ALIGNED ? 1 : 8][ALIGNED ? 8 : kSpan];
   const int warp = warp_id(), lane = lane_id();

@@ -85,7 +85,8 @@ def _pack(fmt: str, *layers: nn.Linear) -> mx.MXTensor:
 
 def quantize_model(model: nn.Module, fmt: str = "mxfp8") -> int:
     """Pack the linears of every DiT block of ``model`` in ``fmt`` (``mxfp8``, ``mxfp4`` or
-    ``nvfp4``); returns how many blocks. Call it again after the weights change."""
+    ``nvfp4``), on the device they are on; returns how many blocks. Call it again after the
+    weights change or move."""
     from avgen_b200.models.blocks import DiTBlock
 
     mx.block_size(fmt)  # raises on an unknown format
@@ -167,6 +168,9 @@ def quantized_block_forward(block: nn.Module, hidden: torch.Tensor, combined: to
     if torch.is_grad_enabled():
         raise RuntimeError("a quantised block has no gradient; run it under torch.no_grad() or call restore_model first")
     p = block.quantized
+    if p.qkv.device != hidden.device:
+        raise RuntimeError(f"packed weights are on {p.qkv.device}, the input on {hidden.device}: call quantize_model after "
+                           "moving the model")
     b, length, w = hidden.shape
     fmt, eps = p.fmt, block.attention_norm.eps or 1e-6
     groups, per = None, length

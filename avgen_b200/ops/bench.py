@@ -7,6 +7,7 @@
     python -m avgen_b200.ops.bench trace --L 16384 --H 20 --pass bwd   # SM-clock timeline of CTA 0
     python -m avgen_b200.ops.bench ring --L 16384 --world 4          # one CP rank's ring attention, emulated
     python -m avgen_b200.ops.bench zero --numel 268435456            # sharded AdamW step on a one-rank group
+    python -m avgen_b200.ops.bench mx --fmt nvfp4 --m 65536 --n 20480 --k 2560   # block-scaled operators
 
 Times come from CUDA events on the launching stream after warm-up, with a
 synchronize on both sides; each line also reports the library equivalent
@@ -241,6 +242,34 @@ def bench_ring(length: int, heads: int, world: int, iters: int, once: bool) -> N
           f"| bwd ({world} launches) {t_b:.3f} ms ({2.5 * flops / t_b / 1e9:.0f} TF/s counted)")
 
 
+def bench_mx(fmt: str, m: int, n: int, k: int, iters: int, once: bool) -> None:
+    """The block-scaled operators on bf16 activations [m, k] and a weight [n, k]."""
+    from avgen_b200.ops import microscale as mx
+
+    x, update = torch.randn(m, k, device="cuda").bfloat16(), torch.randn(m, k, device="cuda").bfloat16()
+    levels = 0.1 * torch.randn(2, 3, k, device="cuda")
+    groups = torch.randint(0, 2, (m,), device="cuda", dtype=torch.int32)
+    norm_weight = torch.ones(k, device="cuda")
+    a, b = mx.quantize(x, fmt), mx.quantize(torch.randn(n, k, device="cuda"), fmt)
+    calls = {
+        "quantize": (lambda: mx.quantize(x, fmt), 2 * x.numel() + a.nbytes),
+        "dequantize": (lambda: mx.dequantize(a), 2 * x.numel() + a.nbytes),
+        "add_rmsnorm_mod, plain": (lambda: mx.add_rmsnorm_mod(x, update, norm_weight, fmt=fmt), 6 * x.numel() + a.nbytes),
+        "add_rmsnorm_mod, 2 levels": (lambda: mx.add_rmsnorm_mod(x, update, norm_weight, levels[:, 0], levels[:, 1],
+                                                                 gate=levels[:, 2], groups=groups, fmt=fmt),
+                                      6 * x.numel() + a.nbytes),
+        "matmul": (lambda: mx.matmul(a, b), a.nbytes + b.nbytes + 2 * m * n),
+    }
+    for name, (call, size) in calls.items():
+        if once:
+            call()
+            continue
+        t = _time(call, iters)
+        rate = f", {2.0 * m * n * k / t / 1e9:.0f} TF/s" if name == "matmul" else ""
+        print(f"{fmt} {m} x {k} {name}: {t * 1e3:.1f} us, {size / t / 1e6:.0f} GB/s{rate}")
+    torch.cuda.synchronize()
+
+
 def main() -> None:
     p = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
     sub = p.add_subparsers(dest="op", required=True)
@@ -267,7 +296,13 @@ def main() -> None:
     z = sub.add_parser("zero")
     z.add_argument("--numel", type=int, default=268435456)
     z.add_argument("--once", action="store_true")
-    for s in (a, g, r, z):
+    x = sub.add_parser("mx")
+    x.add_argument("--fmt", choices=("mxfp8", "mxfp4", "nvfp4"), default="nvfp4")
+    x.add_argument("--m", type=int, default=16384)
+    x.add_argument("--n", type=int, default=7680)
+    x.add_argument("--k", type=int, default=2560)
+    x.add_argument("--once", action="store_true")
+    for s in (a, g, r, z, x):
         s.add_argument("--iters", type=int, default=10)
     args = p.parse_args()
     if getattr(args, "bwd", None):
@@ -283,6 +318,8 @@ def main() -> None:
         bench_ring(args.L, args.H, args.world, args.iters, args.once)
     elif args.op == "zero":
         bench_zero(args.numel, args.iters, args.once)
+    elif args.op == "mx":
+        bench_mx(args.fmt, args.m, args.n, args.k, args.iters, args.once)
     else:
         bench_gemm(args.m, args.n, args.k, args.iters, args.once, args.gated)
     from avgen_b200.ops._ext import check_errors

@@ -305,6 +305,8 @@ def test_device_refusals() -> None:
         (lambda: mx.quantize(x, "nvfp4", global_scale=torch.ones(1)), "CUDA|device"),
         (lambda: mx.quantize(x, "nvfp4", global_scale=torch.ones(2, device=DEV)), "one fp32 value"),
         (lambda: mx.dequantize(a, torch.float64), "bf16, fp16 or fp32"),
+        (lambda: mx.add_rmsnorm_mod(torch.ones(2, 65537, device=DEV), None, None), "at most 65536 columns"),
+        (lambda: mx.matmul(a, mx.MXTensor(a.codes[:, 16:].t().contiguous().t(), a.scales, "nvfp4", 32)), "differ|contiguous"),
         (lambda: mx.matmul(a, a, bias=torch.ones(3, device=DEV)), "bias must be"),
         (lambda: mx.matmul(a, a, bias=torch.ones(4, device=DEV).half()), "fp32"),
         (lambda: mx.matmul(a, a, out_dtype=torch.int32), "bf16, fp16 or fp32"),

@@ -160,6 +160,16 @@ def test_gpu_block_stays_near_the_fp32_block(fmt: str, ffn: str, form: str) -> N
 
 
 @pytest.mark.gpu
+def test_gpu_block_refuses_weights_packed_elsewhere() -> None:
+    block = _block()
+    hidden, kwargs = _inputs("sample", "cuda", torch.bfloat16)
+    quantize_model(block, "mxfp8")
+    block.cuda()
+    with torch.no_grad(), pytest.raises(RuntimeError, match="after moving the model"):
+        block(hidden, **kwargs)
+
+
+@pytest.mark.gpu
 def test_gpu_model_samples_quantised() -> None:
     from dataclasses import asdict
 
