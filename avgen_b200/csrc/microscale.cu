@@ -537,16 +537,16 @@ struct Chunk {
     } else {
       const int lane = lane_id();
       const T* at = from.row + base + lane;
-      float v[kNormLane];
+      T v[kNormLane];
       if (from.row != nullptr && base + kNormSpan <= cols) {  // a whole chunk: no bounds
 #pragma unroll
-        for (int e = 0; e < kNormLane; ++e) v[e] = to_float(at[32 * e]);
+        for (int e = 0; e < kNormLane; ++e) v[e] = at[32 * e];
       } else {
         const int end = from.row != nullptr ? cols - base - lane : 0;
 #pragma unroll
-        for (int e = 0; e < kNormLane; ++e) v[e] = 32 * e < end ? to_float(at[32 * e]) : from.other;
+        for (int e = 0; e < kNormLane; ++e) v[e] = 32 * e < end ? at[32 * e] : from_float<T>(from.other);
       }
-      r.pack(v);
+      memcpy(r.w, v, sizeof(v));
     }
   }
   __device__ __forceinline__ void store(T* row, int base, int cols) const {
@@ -617,7 +617,7 @@ __global__ void __launch_bounds__(CHUNKS == 8 ? 1024 : 512, CHUNKS <= 2 ? 2 : 1)
   if (row < rows) request(row);
   int turn = 0;
   for (; row < rows; row += step) {
-    float v[CHUNKS][kNormLane];
+    __align__(16) float v[CHUNKS][kNormLane];
     const NormRow<float, ALIGNED> gate(d.gate, next_b * d.gate_stride, 1.f);
     const NormRow<float, ALIGNED> scale(d.scale, next_b * d.mod_stride, 0.f);
     const NormRow<float, ALIGNED> shift(d.shift, next_b * d.mod_stride, 0.f);
@@ -693,7 +693,12 @@ __global__ void __launch_bounds__(CHUNKS == 8 ? 1024 : 512, CHUNKS <= 2 ? 2 : 1)
         for (int e = 0; e < kNormLane; ++e) stage[32 * e + lane] = v[i][e];
         __syncwarp();
 #pragma unroll
-        for (int e = 0; e < kNormLane; ++e) v[i][e] = c0 + e < d.W ? stage[lane * kNormLane + e] : 0.f;
+        for (int e = 0; e < kNormLane; e += 4)
+          *reinterpret_cast<float4*>(v[i] + e) = *reinterpret_cast<const float4*>(stage + lane * kNormLane + e);
+        if (at + kNormSpan > d.W) {
+#pragma unroll
+          for (int e = 0; e < kNormLane; ++e) v[i][e] = c0 + e < d.W ? v[i][e] : 0.f;
+        }
       } else if (c0 >= d.W) {  // 0 * (a statistic that overflowed) is not 0
 #pragma unroll
         for (int e = 0; e < kNormLane; ++e) v[i][e] = 0.f;
