@@ -582,7 +582,7 @@ struct Chunk {
 // modulation and scaling stay in fp32 until the codes.
 // MODULATED = false leaves gate, scale and shift out: their neutral values would cost registers and so CTAs in flight.
 template <typename T, int FMT, int CHUNKS, bool WARP_ROWS, bool ALIGNED, bool MODULATED>
-__global__ void __launch_bounds__(CHUNKS == 8 ? 1024 : 512, CHUNKS <= 2 ? 2 : 1) mx_add_rmsnorm_kernel(MxNormDesc d, PackedRows p) {
+__global__ void __launch_bounds__(CHUNKS == 8 ? 1024 : WARP_ROWS ? 128 : 512, WARP_ROWS ? (CHUNKS <= 2 ? 8 : 5) : CHUNKS <= 2 ? 2 : 1) mx_add_rmsnorm_kernel(MxNormDesc d, PackedRows p) {
   extern __shared__ __align__(16) float stages[];  // 256 per warp, unaligned rows only
   __shared__ float red[2][32];
   const int warp = warp_id(), lane = lane_id();
@@ -801,7 +801,7 @@ void add_rmsnorm_aligned(const MxNormDesc& d, const PackedRows& p, cudaStream_t 
   const int spans = static_cast<int>((d.W + kNormSpan - 1) / kNormSpan);
   if (spans == 1) return add_rmsnorm_as<T, FMT, 1, true, ALIGNED>(d, p, 4, stream);
   if (spans == 2) return add_rmsnorm_as<T, FMT, 2, true, ALIGNED>(d, p, 4, stream);
-  if (spans <= 4) return add_rmsnorm_as<T, FMT, 4, true, ALIGNED>(d, p, 4, stream);
+  if (spans == 3) return add_rmsnorm_as<T, FMT, 3, true, ALIGNED>(d, p, 4, stream);
   if (spans <= 32) return add_rmsnorm_as<T, FMT, 2, false, ALIGNED>(d, p, (spans + 1) / 2, stream);
   if (spans <= 64) return add_rmsnorm_as<T, FMT, 4, false, ALIGNED>(d, p, (spans + 3) / 4, stream);
   add_rmsnorm_as<T, FMT, 8, false, ALIGNED>(d, p, (spans + 7) / 8, stream);
