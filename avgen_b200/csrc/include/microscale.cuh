@@ -16,6 +16,8 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 namespace avgen {
 
 enum MxFormat : int { kMxFp8 = 0, kMxFp4 = 1, kNvFp4 = 2 };
@@ -31,10 +33,6 @@ __host__ __device__ constexpr long mx_scale_tiles(int fmt, long cols) {
 }
 __host__ __device__ constexpr long mx_scale_bytes(int fmt, long rows, long cols) {
   return (rows + 127) / 128 * mx_scale_tiles(fmt, cols) * 512;
-}
-// Byte offset of the four scales of tile `tile` in row `row` (block b of the tile: + b).
-__host__ __device__ constexpr long mx_scale_word(long row, long tile, long tiles) {
-  return (row / 128 * tiles + tile) * 512 + row % 32 * 16 + row % 128 / 32 * 4;
 }
 
 #ifdef __CUDACC__
@@ -65,16 +63,6 @@ __device__ __forceinline__ uint32_t cvt_e4m3x2(float lo, float hi) {
 __device__ __forceinline__ uint32_t cvt_e4m3x4(float a, float b, float c, float d) {
   return cvt_e4m3x2(a, b) | (cvt_e4m3x2(c, d) << 16);
 }
-// Two e2m1 codes, `lo` in the low half of the byte.
-__device__ __forceinline__ uint32_t cvt_e2m1x2(float lo, float hi) {
-  uint32_t r;
-  asm("{\n\t.reg .b8 b0;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
-      "mov.b32 %0, {b0, b0, b0, b0};\n\t}"
-      : "=r"(r)
-      : "f"(lo), "f"(hi));
-  return r & 0xffu;
-}
 // Eight e2m1 codes, v[0] in the lowest four bits.
 __device__ __forceinline__ uint32_t cvt_e2m1x8(const float* v) {
   uint32_t r;
@@ -94,11 +82,6 @@ __device__ __forceinline__ float2 e4m3x2_to_float2(uint32_t two) {
   return __half22float2(*reinterpret_cast<__half2*>(&h));
 }
 __device__ __forceinline__ float e4m3_to_float(uint32_t byte) { return e4m3x2_to_float2(byte & 0xffu).x; }
-__device__ __forceinline__ float e2m1_to_float(uint32_t code) {
-  const float a = (code & 6u) != 0u ? __uint_as_float((126u + ((code >> 1) & 3u)) << 23 | (code & 1u) << 22)
-                                    : (code & 1u) * 0.5f;
-  return (code & 8u) != 0u ? -a : a;
-}
 // Values of the eight e2m1 codes of a word.
 __device__ __forceinline__ void e2m1x8_to_float(uint32_t w, float* v) {
   uint32_t h[4];
@@ -170,6 +153,26 @@ template <typename T> __device__ __forceinline__ T from_float(float v);
 template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+// Two 16-bit values of a word.
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void unpack2(uint32_t w, float& lo, float& hi) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    lo = __uint_as_float(w << 16), hi = __uint_as_float(w & 0xffff0000u);
+  } else {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    lo = f.x, hi = f.y;
+  }
+}
 #endif  // __CUDACC__
 
 }  // namespace avgen
