@@ -905,6 +905,18 @@ void p2p_copy_py(int64_t dst, int64_t src, int64_t bytes) {
 at::Tensor mx_empty(at::IntArrayRef sizes, at::ScalarType type, at::Device device) {
   return at::detail::empty_cuda(sizes, type, device, c10::nullopt);
 }
+// Codes and scales of a packed tensor, two views of one allocation: they live and die together.
+std::pair<at::Tensor, at::Tensor> mx_empty_packed(int fmt, long rows, long cols, at::Device device) {
+  const long row_bytes = mx_row_bytes(fmt, cols), scale_bytes = mx_scale_bytes(fmt, rows, cols);
+  const long start = (rows * row_bytes + 511) / 512 * 512;  // scales on a tile boundary, as an allocation of their own
+  at::Tensor all = mx_empty({start + scale_bytes}, at::kByte, device);
+  at::Tensor scales = at::detail::make_tensor<c10::TensorImpl>(c10::TensorImpl::VIEW, c10::Storage(all.storage()),
+                                                               all.key_set(), all.dtype());
+  scales.unsafeGetTensorImpl()->set_storage_offset(start);
+  scales.unsafeGetTensorImpl()->set_sizes_contiguous({scale_bytes});
+  all.unsafeGetTensorImpl()->set_sizes_contiguous({rows, row_bytes});
+  return {all, scales};
+}
 int mx_dtype(at::ScalarType t, const char* what) {
   if (t == at::kBFloat16) return kMxBf16;
   if (t == at::kHalf) return kMxFp16;
@@ -956,8 +968,7 @@ std::tuple<at::Tensor, at::Tensor, OptT, int> mx_quantize(const at::Tensor& x, i
   d.x = rows.data_ptr();
   TORCH_CHECK(d.rows < (1L << 31) - 256 && d.cols < (1L << 25), "quantize: too many rows or columns");
   d.ldx = rows.stride(0);
-  at::Tensor codes = mx_empty({d.rows, mx_row_bytes(d.fmt, d.cols)}, at::kByte, x.device());
-  at::Tensor scales = mx_empty({mx_scale_bytes(d.fmt, d.rows, d.cols)}, at::kByte, x.device());
+  auto [codes, scales] = mx_empty_packed(d.fmt, d.rows, d.cols, x.device());
   d.codes = codes.data_ptr<uint8_t>();
   d.scales = scales.data_ptr<uint8_t>();
   d.g = mx_global(g, x, "quantize: global_scale");
@@ -1058,8 +1069,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> mx_add_rmsnorm(const at::Tensor& 
     TORCH_CHECK(d.groups != nullptr || mod_rows * d.rows_per_batch >= d.rows,
                 "add_rmsnorm: modulation rows do not cover x");
   }
-  at::Tensor codes = mx_empty({d.rows, mx_row_bytes(d.fmt, d.W)}, at::kByte, x.device());
-  at::Tensor scales = mx_empty({mx_scale_bytes(d.fmt, d.rows, d.W)}, at::kByte, x.device());
+  auto [codes, scales] = mx_empty_packed(d.fmt, d.rows, d.W, x.device());
   d.codes = codes.data_ptr<uint8_t>();
   d.scales = scales.data_ptr<uint8_t>();
   if (d.rows > 0) mx_add_rmsnorm_launch(d, cur_stream());

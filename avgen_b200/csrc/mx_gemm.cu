@@ -61,8 +61,9 @@ constexpr int kSmemLimit = 232448;
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = 64 + 32 * kEpiWarps;
 
+// One staged k-block and the TMEM columns of its scales.
 template <int FMT, int BN, int CTAS>
-struct Cfg {
+struct StageCfg {
   static constexpr int SF_TILES = FMT == kNvFp4 ? 4 : FMT == kMxFp4 ? 2 : 1;  // scale tiles per k-block
   static constexpr int B_ROWS = BN / CTAS;
   static constexpr int A_BYTES = kBM * kRowBytes;
@@ -72,16 +73,21 @@ struct Cfg {
   static constexpr int SFB_BYTES = SFB_GROUPS * SFA_BYTES;  // of all BN rows, in both CTAs
   static constexpr int TX_BYTES = A_BYTES + B_BYTES + SFA_BYTES + SFB_BYTES;
   static constexpr int STAGE_BYTES = (TX_BYTES + 1023) / 1024 * 1024;
+  static constexpr int SF_COLS = (SF_TILES * 4 * (1 + SFB_GROUPS) + 31) / 32 * 32;
+};
+
+template <int FMT, int BN, int CTAS>
+struct Cfg : StageCfg<FMT, BN, CTAS> {
+  using S = StageCfg<FMT, BN, CTAS>;
   static constexpr int OUT_BYTES = kEpiWarps * kBoxBytes;
-  static constexpr int STAGES = std::min(8, (kSmemLimit - 2048 - OUT_BYTES) / STAGE_BYTES);
-  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + OUT_BYTES + 1024 + 256;
+  static constexpr int STAGES = std::min(8, (kSmemLimit - 2048 - OUT_BYTES) / S::STAGE_BYTES);
+  static constexpr int SMEM_BYTES = STAGES * S::STAGE_BYTES + OUT_BYTES + 1024 + 256;
   // TMEM: two accumulators and the scales of one k-block. Two 256-column accumulators
   // leave no room for scales, so the second starts inside the first: the epilogue reads
   // the shared columns first and hands them over, and the next tile's products wait for
   // that instead of for a free accumulator.
-  static constexpr int SF_COLS = (SF_TILES * 4 * (1 + SFB_GROUPS) + 31) / 32 * 32;
-  static constexpr bool OVERLAP = 2 * BN + SF_COLS > 512;
-  static constexpr int ACC1 = OVERLAP ? 512 - SF_COLS - BN : BN;
+  static constexpr bool OVERLAP = 2 * BN + S::SF_COLS > 512;
+  static constexpr int ACC1 = OVERLAP ? 512 - S::SF_COLS - BN : BN;
   static constexpr int SF_COL = ACC1 + BN;
 };
 
@@ -134,7 +140,7 @@ __device__ __forceinline__ void copy_scales(uint32_t taddr, uint64_t desc) {
 // addition (addresses are below 2^18 bytes, so the 14-bit field does not carry).
 template <int FMT, int BN, int CTAS>
 struct Issuer {
-  using C = Cfg<FMT, BN, CTAS>;
+  using C = StageCfg<FMT, BN, CTAS>;
   static constexpr int SFB_TILES = C::SFB_GROUPS;
   static constexpr int PER = kSteps / C::SF_TILES;  // products per scale tile
   uint64_t a, b, sfa, sfb;
@@ -538,7 +544,7 @@ constexpr int kMaxSplits = 8;  // CTAs of a portable cluster
 
 template <int FMT, int MT>
 struct SplitCfg {
-  using C = Cfg<FMT, MT, 1>;
+  using C = StageCfg<FMT, MT, 1>;
   static constexpr int CTAS_PER_SM = MT <= 32 ? 2 : 1;
   static constexpr int STAGES = std::min(8, (kSmemLimit / CTAS_PER_SM - 2048) / C::STAGE_BYTES);
   static constexpr int SMEM_BYTES = STAGES * C::STAGE_BYTES + 1024 + 256;
