@@ -398,6 +398,7 @@ __global__ void __launch_bounds__(32 * kSmallWarps) mx_quantize_small_kernel(MxQ
   __shared__ uint32_t warp_max[kSmallWarps];
   __shared__ uint32_t cta_max[kSmallCtas];  // every CTA writes its word in every CTA
   const int warp = warp_id(), lane = lane_id(), ctas = gridDim.x;
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // waited for below: every CTA has started
   const int unit = blockIdx.x * kSmallWarps + warp;
   const long row = unit / segments, base = static_cast<long>(unit % segments) * kSpan, c0 = base + lane * kLane;
   const T* x = reinterpret_cast<const T*>(d.x) + row * d.ldx;
@@ -415,6 +416,7 @@ __global__ void __launch_bounds__(32 * kSmallWarps) mx_quantize_small_kernel(MxQ
   const uint32_t m = __reduce_max_sync(kAllLanes, finite_max(r));
   if (lane == 0) warp_max[warp] = m;
   __syncthreads();
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   if (warp == 0) {
     const uint32_t all = __reduce_max_sync(kAllLanes, warp_max[lane % kSmallWarps]);
     if (lane < ctas) {

@@ -268,6 +268,11 @@ __device__ __forceinline__ void free_tmem(uint32_t taddr) {
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(taddr));
 }
 
+// mbar_wait with one answer for the whole warp.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err, int code) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, err, code));
+}
+
 // After an abort: copies still in flight land well within a millisecond.
 __device__ __forceinline__ void let_copies_land() {
   const uint64_t t0 = globaltimer();
@@ -382,22 +387,21 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = *tmem_slot;
 
   // Both issuing roles run warp-uniform with one elected thread: from a divergent branch
-  // each TMA or tcgen05 instruction takes several times as long to issue (mxfp8 32768 x
+  // each TMA or tcgen05 instruction takes several times as long to issue (mxfp8 16384 x
   // 5120 x 5120: products issued by `if (lane == 0)` ran at 2.2 instead of 2.8 PFLOP/s).
+  // A wait that runs out may do so for some lanes only, so no lane leaves its loop early:
+  // an aborted one goes on without waiting or issuing.
   if (warp == 0) {
     int stage = 0;
     uint32_t phase = 0;
     bool aborted = false;
     const uint32_t bar0 = CTAS == 2 ? map_to_rank(smem_u32(full), 0) : smem_u32(full);
-    for (int t = first; t < num_tiles && !aborted; t += step) {
+    for (int t = first; t < num_tiles; t += step) {
       int tm, tn;
       tile_at(t, num_m, num_n, tm, tn);
       for (int kb = 0; kb < args.num_kb; ++kb) {
-        if (!mbar_wait(&empty[stage], phase ^ 1, abort_flag, args.err, kErrTimeoutProducer)) {
-          aborted = true;
-          break;
-        }
-        if (elect_one()) {
+        if (!aborted) aborted = !mbar_wait(&empty[stage], phase ^ 1, abort_flag, args.err, kErrTimeoutProducer);
+        if (elect_one() && !aborted) {
           uint8_t* sa = smem + stage * C::STAGE_BYTES;
           uint8_t* sb = sa + C::A_BYTES;
           uint8_t* sfa = sb + C::B_BYTES;
@@ -425,19 +429,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t phase = 0;
       bool aborted = false;
       int i = 0;  // tiles done by this CTA
-      for (int t = first; t < num_tiles && !aborted; t += step, ++i) {
+      for (int t = first; t < num_tiles; t += step, ++i) {
         const int acc = i & 1;
         // the tile that must have been read (its shared columns, or all of it) before this one
         const int before = C::OVERLAP ? i - 1 : i - 2;
-        if (before >= 0 && !mbar_wait(&tempty[before & 1], (before >> 1) & 1, abort_flag, args.err, kErrTimeoutMma)) break;
+        if (before >= 0 && !aborted)
+          aborted = !mbar_wait(&tempty[before & 1], (before >> 1) & 1, abort_flag, args.err, kErrTimeoutMma);
         tc_fence_after();
         for (int kb = 0; kb < args.num_kb; ++kb) {
-          if (!mbar_wait(&full[stage], phase, abort_flag, args.err, kErrTimeoutMma)) {
-            aborted = true;
-            break;
-          }
+          if (!aborted) aborted = !mbar_wait(&full[stage], phase, abort_flag, args.err, kErrTimeoutMma);
           tc_fence_after();
-          if (elect_one()) {
+          if (elect_one() && !aborted) {
             issue.block(stage, tmem + acc * C::ACC1, idesc, kb == args.num_kb - 1 ? args.last_steps : kSteps, kb == 0);
             commit<CTAS>(&empty[stage]);
           }
@@ -447,8 +449,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             phase ^= 1;
           }
         }
-        if (aborted) break;
-        if (elect_one()) commit<CTAS>(&tfull[acc]);
+        if (elect_one() && !aborted) commit<CTAS>(&tfull[acc]);
         __syncwarp();
       }
     }
@@ -466,7 +467,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int tm, tn;
       tile_at(t, num_m, num_n, tm, tn);
       const int acc = i & 1;
-      if (!mbar_wait(&tfull[acc], (i >> 1) & 1, abort_flag, args.err, kErrTimeoutEpilogue)) break;
+      if (!warp_wait(&tfull[acc], (i >> 1) & 1, abort_flag, args.err, kErrTimeoutEpilogue)) break;
       tc_fence_after();
       // What this warp has to have read before the next tile's products may start: with
       // overlapping accumulators the shared columns (the first one's last, the second one's
@@ -592,14 +593,12 @@ __global__ void __launch_bounds__(192, 1)
   const uint32_t tmem = *tmem_slot;
 
   if (warp == 0) {
+    bool aborted = false;
     for (int kb = kb0, i = 0; kb < kb1; ++kb, ++i) {
       const int stage = i % S::STAGES;
-      if (i >= S::STAGES &&
-          !mbar_wait(&empty[stage], (i / S::STAGES - 1) & 1, abort_flag, args.err, kErrTimeoutProducer)) {
-        let_copies_land();
-        break;
-      }
-      if (elect_one()) {
+      if (i >= S::STAGES && !aborted)
+        aborted = !mbar_wait(&empty[stage], (i / S::STAGES - 1) & 1, abort_flag, args.err, kErrTimeoutProducer);
+      if (elect_one() && !aborted) {
         uint8_t* sw = smem + stage * C::STAGE_BYTES;
         uint8_t* sx = sw + C::A_BYTES;
         uint8_t* sfw = sx + C::B_BYTES;
@@ -612,26 +611,24 @@ __global__ void __launch_bounds__(192, 1)
       }
       __syncwarp();
     }
+    if (aborted) let_copies_land();
   } else if (warp == 1) {
     constexpr uint32_t idesc = mx_idesc<FMT>(128, MT);
     const Issuer<FMT, MT, 1> issue(smem_u32(smem), tmem + MT);
     bool aborted = false;
     for (int kb = kb0, i = 0; kb < kb1; ++kb, ++i) {
       const int stage = i % S::STAGES;
-      if (!mbar_wait(&full[stage], (i / S::STAGES) & 1, abort_flag, args.err, kErrTimeoutMma)) {
-        aborted = true;
-        break;
-      }
+      if (!aborted) aborted = !mbar_wait(&full[stage], (i / S::STAGES) & 1, abort_flag, args.err, kErrTimeoutMma);
       tc_fence_after();
-      if (elect_one()) {
+      if (elect_one() && !aborted) {
         issue.block(stage, tmem, idesc, kb == args.num_kb - 1 ? args.last_steps : kSteps, kb == kb0);
         mma_commit(&empty[stage]);
       }
       __syncwarp();
     }
-    if (!aborted && elect_one()) mma_commit(tfull);
+    if (elect_one() && !aborted) mma_commit(tfull);
     __syncwarp();
-  } else if (mbar_wait(tfull, 0, abort_flag, args.err, kErrTimeoutEpilogue)) {
+  } else if (warp_wait(tfull, 0, abort_flag, args.err, kErrTimeoutEpilogue)) {
     tc_fence_after();
     const int q = warp & 3;
     const int lane_n = q * 32 + lane, n = n0 + lane_n;
