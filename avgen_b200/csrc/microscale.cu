@@ -13,8 +13,8 @@
 //   quantise   mxfp8 83 (6.1), mxfp4 73 (5.8), nvfp4 with a given tensor scale 77 (5.6),
 //              with its own 134; fp32 13824 x 5120 to mxfp4 54 (6.0)
 //   read back  mxfp8 85 (6.0), 4 bits 74 (5.8)
-//   norm       to mxfp8 187 (6.3), with two modulation levels 212 (5.6); 16387 x 5120 97
-//              (6.1); 20000 x 5001, whose rows are not aligned, 233 (3.0)
+//   norm       to mxfp8 192 (6.1), with two modulation levels 221 (5.3); 16387 x 5120 99
+//              (5.9); 20000 x 5001, whose rows are not aligned, 227 (3.1)
 #include <algorithm>
 
 #include "include/host_utils.h"
@@ -569,6 +569,15 @@ struct Chunk {
   __device__ __forceinline__ Pair pair(int e) const { return {__uint_as_float(r.w[e]), __uint_as_float(r.w[e + 1])}; }
 };
 
+// 1 / sqrt(x), the hardware's approximation improved by a Newton step: an error of a row's
+// factor moves all of the row's values towards the same side of their roundings. Outside
+// the step's range (0, infinity, NaN) the approximation stands.
+__device__ __forceinline__ float inverse_root(float x) {
+  const float r = rsqrtf(x);
+  const float e = fmaf(-x * r, r, 1.f);
+  return fabsf(e) < 0.5f ? fmaf(0.5f * r, e, r) : r;
+}
+
 // A row is held in registers, CHUNKS x 8 columns per lane, between its sum of squares
 // and its store: x and the update are read once. Rows of up to 1024 columns take one
 // warp each (WARP_ROWS) and no barrier; longer ones a CTA, with one barrier per row. The
@@ -582,7 +591,9 @@ struct Chunk {
 // rows per token from L1 (12 of the 19 bytes a value moves through it). Registers decide
 // how many rows are in flight: rows of up to 8192 columns keep to 64 (two modulation
 // levels 244 -> 228 us), and MODULATED = false leaves gate, scale and shift out, whose
-// neutral values would cost 20 (235 -> 186 us).
+// neutral values would cost 20 (235 -> 186 us). The row's factor to the last bit or so
+// costs 4 us (187 -> 192) and keeps the share of values that round otherwise than in 64
+// bits at that of the same formula in plain fp32.
 template <typename T, int FMT, int CHUNKS, bool WARP_ROWS, bool ALIGNED, bool MODULATED>
 __global__ void __launch_bounds__(CHUNKS == 8 ? 1024 : WARP_ROWS ? 128 : 512, WARP_ROWS ? (CHUNKS <= 2 ? 8 : 5) : CHUNKS <= 2 ? 2 : 1) mx_add_rmsnorm_kernel(MxNormDesc d, PackedRows p) {
   extern __shared__ __align__(16) float stages[];  // 256 per warp, unaligned rows only
@@ -591,7 +602,9 @@ __global__ void __launch_bounds__(CHUNKS == 8 ? 1024 : WARP_ROWS ? 128 : 512, WA
   const int warps = WARP_ROWS ? 1 : blockDim.x >> 5;  // of a row
   const int place = WARP_ROWS ? 0 : warp;
   const float g = FMT == kNvFp4 && d.g != nullptr ? *d.g : 1.f;
-  const float six_g = 6.f * g, inv_six_g = __frcp_rn(six_g), inv_w = 1.f / static_cast<float>(d.W);
+  const float six_g = 6.f * g, inv_six_g = __frcp_rn(six_g);
+  const float width = static_cast<float>(d.W), inv_w = __frcp_rn(width);  // 1 / W = inv_w + inv_w_rest
+  const float inv_w_rest = fmaf(-width, inv_w, 1.f) * inv_w;
   const int padded = static_cast<int>((d.rows + 127) / 128 * 128), rows = static_cast<int>(d.rows);
   const int step = WARP_ROWS ? gridDim.x * (blockDim.x >> 5) : gridDim.x;
   int row = WARP_ROWS ? blockIdx.x * (blockDim.x >> 5) + warp : blockIdx.x;
@@ -664,11 +677,14 @@ __global__ void __launch_bounds__(CHUNKS == 8 ? 1024 : WARP_ROWS ? 128 : 512, WA
     if constexpr (!WARP_ROWS) {
       if (lane == 0) red[turn][warp] = sum;
       __syncthreads();  // one per row: the next row's sums go to the other buffer
-      sum = 0.f;
-      for (int i = 0; i < warps; ++i) sum += red[turn][i];
+      constexpr int MOST = CHUNKS == 8 ? 32 : 16;  // warps; each run of as many lanes adds them up
+      const int from = lane % MOST;
+      sum = from < warps ? red[turn][from] : 0.f;
+#pragma unroll
+      for (int o = MOST / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(kAllLanes, sum, o);
       turn ^= 1;
     }
-    const float r = rsqrtf(fmaf(sum, inv_w, d.eps));
+    const float r = inverse_root(fmaf(sum, inv_w, fmaf(sum, inv_w_rest, d.eps)));
     uint8_t* codes = p.codes_of(row);
     uint8_t* scales = p.scales_of(row);
 #pragma unroll
