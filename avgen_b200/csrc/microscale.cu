@@ -11,8 +11,9 @@
 // Measured on a B200 whose plain copy runs at 6.56 TB/s; 65536 x 2560 bf16 where no size
 // is given, bytes counted once each (us, TB/s):
 //   quantise   mxfp8 83 (6.1), mxfp4 73 (5.8), nvfp4 with a given tensor scale 77 (5.6),
-//              with its own 134; fp32 13824 x 5120 to mxfp4 54 (6.0)
-//   read back  mxfp8 85 (6.0), 4 bits 74 (5.8)
+//              with its own 134; fp32 13824 x 5120 to mxfp4 54 (6.0); 20000 x 5001 to
+//              mxfp4, rows not aligned, 69 (3.7)
+//   read back  mxfp8 85 (6.0), 4 bits 74 (5.8); 20000 x 5001 from mxfp4 60 (4.2)
 //   norm       to mxfp8 192 (6.1), with two modulation levels 221 (5.3); 16387 x 5120 99
 //              (5.9); 20000 x 5001, whose rows are not aligned, 227 (3.1)
 #include <algorithm>
@@ -193,8 +194,8 @@ struct LanePlace {
 // Quantises and stores a lane's N values (zero past the row's end), whose largest
 // magnitude is `m`. Called by whole warps.
 template <int FMT, int N>
-__device__ __forceinline__ void store_packed(const LanePlace<FMT, N>& at, uint8_t* codes, uint8_t* scales, float (&v)[N],
-                                             uint32_t m, float g, float six_g, float inv_six_g) {
+__device__ __forceinline__ void store_packed(const LanePlace<FMT, N>& at, uint8_t* codes, uint8_t* scales,
+                                             float (&v)[N], uint32_t m, float g, float six_g, float inv_six_g) {
   constexpr int LANES = LanePlace<FMT, N>::LANES;
   if constexpr (LANES >= 2) m = max(m, __shfl_xor_sync(kAllLanes, m, 1));
   if constexpr (LANES >= 4) m = max(m, __shfl_xor_sync(kAllLanes, m, 2));
@@ -219,8 +220,8 @@ __device__ __forceinline__ void store_packed(const LanePlace<FMT, N>& at, uint8_
 }
 
 // The (zero) scales of a row past the tensor, inside its last 128-row group.
-__device__ __forceinline__ void store_pad_scales(const PackedRows& p, long row, long first_tile, long end_tile, int lane,
-                                                 int lanes) {
+__device__ __forceinline__ void store_pad_scales(const PackedRows& p, long row, long first_tile, long end_tile,
+                                                 int lane, int lanes) {
   for (long t = first_tile + lane; t < min(end_tile, p.tiles); t += lanes)
     *reinterpret_cast<uint32_t*>(p.scales_of(row) + t * 512) = 0u;
 }
@@ -236,10 +237,14 @@ struct Unaligned {
   T v[kLane];  // columns base + 32 j + lane
 
   __device__ __forceinline__ void load(const T* row, long base, long cols) {
+    const T* at = row + base + lane_id();
+    if (base + kSpan <= cols) {  // no bounds inside the row
 #pragma unroll
-    for (int j = 0; j < kLane; ++j) {
-      const long c = base + 32 * j + lane_id();
-      v[j] = c < cols ? row[c] : from_float<T>(0.f);
+      for (int j = 0; j < kLane; ++j) v[j] = at[32 * j];
+    } else {
+      const int end = static_cast<int>(cols - base) - lane_id();
+#pragma unroll
+      for (int j = 0; j < kLane; ++j) v[j] = 32 * j < end ? at[32 * j] : from_float<T>(0.f);
     }
   }
   __device__ __forceinline__ void to_lanes(T* stage, Raw<T, kLane>& r) const {
@@ -257,10 +262,16 @@ struct Unaligned {
     for (int i = 0; i < r.WORDS; i += 4)
       reinterpret_cast<uint4*>(stage + lane_id() * kLane)[i / 4] = *reinterpret_cast<const uint4*>(r.w + i);
     __syncwarp();
+    T* at = row + base + lane_id();
+    const T* from = stage + lane_id();
+    if (base + kSpan <= cols) {
 #pragma unroll
-    for (int j = 0; j < kLane; ++j) {
-      const long c = base + 32 * j + lane_id();
-      if (c < cols) row[c] = stage[32 * j + lane_id()];
+      for (int j = 0; j < kLane; ++j) at[32 * j] = from[32 * j];
+    } else {
+      const int end = static_cast<int>(cols - base) - lane_id();
+#pragma unroll
+      for (int j = 0; j < kLane; ++j)
+        if (32 * j < end) at[32 * j] = from[32 * j];
     }
   }
 };
@@ -330,8 +341,9 @@ __global__ void __launch_bounds__(256) mx_amax_kernel(MxQuantDesc d) {
 // rate is most of what an SM issues: maxima are taken on the 16-bit values two at a time
 // and scaling two at a time in fp32 (nvfp4 with a given tensor scale 94 -> 79 us).
 template <typename T, int FMT, bool ALIGNED>
-__global__ void __launch_bounds__(256, ALIGNED ? 4 : 2) mx_quantize_kernel(MxQuantDesc d, PackedRows p, int rows_per_cta) {
-  constexpr int UNROLL = ALIGNED && sizeof(T) == 2 ? 4 : 2;
+__global__ void __launch_bounds__(256, 4)
+    mx_quantize_kernel(MxQuantDesc d, PackedRows p, int rows_per_cta) {
+  constexpr int UNROLL = !ALIGNED ? 1 : sizeof(T) == 2 ? 4 : 2;
   __shared__ __align__(16) T stage[ALIGNED ? 1 : 8][ALIGNED ? 8 : kSpan];
   const int warp = warp_id(), lane = lane_id();
   // nvfp4 has just read the whole tensor for its scale: from the end, where L2 still holds it
@@ -381,7 +393,8 @@ __global__ void __launch_bounds__(256, ALIGNED ? 4 : 2) mx_quantize_kernel(MxQua
         store_packed<FMT>(place, p.codes_of(at), p.scales_of(at), v, r[i].amax(), g, six_g, inv_six_g);
       } else {
         constexpr int TILES = kSpan / (4 * mx_block(FMT));
-        store_pad_scales(p, at, static_cast<long>(blockIdx.y) * TILES, static_cast<long>(blockIdx.y + 1) * TILES, lane, 32);
+        const long first_tile = static_cast<long>(blockIdx.y) * TILES;
+        store_pad_scales(p, at, first_tile, first_tile + TILES, lane, 32);
       }
     }
   }
@@ -393,7 +406,8 @@ __global__ void __launch_bounds__(256, ALIGNED ? 4 : 2) mx_quantize_kernel(MxQua
 constexpr int kSmallWarps = 16, kSmallCtas = 8;
 
 template <typename T, bool ALIGNED>
-__global__ void __launch_bounds__(32 * kSmallWarps) mx_quantize_small_kernel(MxQuantDesc d, PackedRows p, int segments) {
+__global__ void __launch_bounds__(32 * kSmallWarps)
+    mx_quantize_small_kernel(MxQuantDesc d, PackedRows p, int segments) {
   __shared__ __align__(16) T stage[ALIGNED ? 1 : kSmallWarps][ALIGNED ? 8 : kSpan];
   __shared__ uint32_t warp_max[kSmallWarps];
   __shared__ uint32_t cta_max[kSmallCtas];  // every CTA writes its word in every CTA
@@ -447,7 +461,7 @@ template <typename T, int FMT, bool ALIGNED>
 __global__ void __launch_bounds__(256) mx_dequantize_kernel(MxDequantDesc d, PackedRows p, int rows_per_cta) {
   constexpr int B = mx_block(FMT);
   constexpr int WORDS = kLane * mx_bits(FMT) / 32;
-  constexpr int UNROLL = ALIGNED ? 4 : 2;
+  constexpr int UNROLL = ALIGNED ? 4 : 1;
   __shared__ __align__(16) T stage[ALIGNED ? 1 : 8][ALIGNED ? 8 : kSpan];
   const int warp = warp_id(), lane = lane_id();
   const long base = static_cast<long>(blockIdx.y) * kSpan;
@@ -595,7 +609,9 @@ __device__ __forceinline__ float inverse_root(float x) {
 // costs 4 us (187 -> 192) and keeps the share of values that round otherwise than in 64
 // bits at that of the same formula in plain fp32.
 template <typename T, int FMT, int CHUNKS, bool WARP_ROWS, bool ALIGNED, bool MODULATED>
-__global__ void __launch_bounds__(CHUNKS == 8 ? 1024 : WARP_ROWS ? 128 : 512, WARP_ROWS ? (CHUNKS <= 2 ? 8 : 5) : CHUNKS <= 2 ? 2 : 1) mx_add_rmsnorm_kernel(MxNormDesc d, PackedRows p) {
+__global__ void __launch_bounds__(CHUNKS == 8 ? 1024 : WARP_ROWS ? 128 : 512,
+                                  WARP_ROWS ? (CHUNKS <= 2 ? 8 : 5) : CHUNKS <= 2 ? 2 : 1)
+    mx_add_rmsnorm_kernel(MxNormDesc d, PackedRows p) {
   extern __shared__ __align__(16) float stages[];  // 256 per warp, unaligned rows only
   __shared__ float red[2][32];
   const int warp = warp_id(), lane = lane_id();
@@ -762,7 +778,8 @@ void quantize_as(const MxQuantDesc& d, const PackedRows& p, cudaStream_t stream)
       attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
       cfg.attrs = &attr;
       cfg.numAttrs = 1;
-      AVGEN_CUDA_CHECK(cudaLaunchKernelEx(&cfg, mx_quantize_small_kernel<T, ALIGNED>, d, p, static_cast<int>(segments)));
+      auto kernel = mx_quantize_small_kernel<T, ALIGNED>;
+      AVGEN_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, d, p, static_cast<int>(segments)));
       return;
     }
     if (d.amax != nullptr)
@@ -788,8 +805,8 @@ void dequantize_as(const MxDequantDesc& d, const PackedRows& p, cudaStream_t str
   const long segments = segments_of(d.cols);
   AVGEN_CHECK(segments <= 65535, "dequantize: too many columns: ", d.cols);
   const int rpc = rows_per_cta(d.rows, segments, num_sms(d.device));
-  mx_dequantize_kernel<T, FMT, ALIGNED>
-      <<<dim3(static_cast<unsigned>((d.rows + rpc - 1) / rpc), static_cast<unsigned>(segments)), 256, 0, stream>>>(d, p, rpc);
+  const dim3 grid(static_cast<unsigned>((d.rows + rpc - 1) / rpc), static_cast<unsigned>(segments));
+  mx_dequantize_kernel<T, FMT, ALIGNED><<<grid, 256, 0, stream>>>(d, p, rpc);
   AVGEN_CUDA_CHECK(cudaGetLastError());
 }
 

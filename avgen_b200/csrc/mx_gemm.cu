@@ -269,7 +269,8 @@ __device__ __forceinline__ void free_tmem(uint32_t taddr) {
 }
 
 // mbar_wait with one answer for the whole warp.
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err, int code) {
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err,
+                                          int code) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, err, code));
 }
 
@@ -343,7 +344,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                    const __grid_constant__ CUtensorMap tmOut, const bool tma_out, const MxArgs args) {
   using C = Cfg<FMT, BN, CTAS>;
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* smem = smem_raw + (1024u - smem_u32(smem_raw) % 1024u) % 1024u;
   uint8_t* smem_out = smem + C::STAGES * C::STAGE_BYTES;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem_out + C::OUT_BYTES);
   uint64_t* empty = full + C::STAGES;
@@ -561,7 +562,7 @@ __global__ void __launch_bounds__(192, 1)
   using S = SplitCfg<FMT, MT>;
   using C = typename S::C;
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* smem = smem_raw + (1024u - smem_u32(smem_raw) % 1024u) % 1024u;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::STAGES * C::STAGE_BYTES);
   uint64_t* empty = full + S::STAGES;
   uint64_t* tfull = empty + S::STAGES;
@@ -707,8 +708,8 @@ __global__ void __launch_bounds__(192, 1)
   }
 }
 
-CUtensorMap encode(CUtensorMapDataType type, int rank, const void* ptr, const cuuint64_t* dims, const cuuint64_t* strides,
-                   const cuuint32_t* box, CUtensorMapSwizzle swizzle, const char* what) {
+CUtensorMap encode(CUtensorMapDataType type, int rank, const void* ptr, const cuuint64_t* dims,
+                   const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle swizzle, const char* what) {
   CUtensorMap map;
   const cuuint32_t estr[3] = {1, 1, 1};
   const CUresult r = tensor_map_encoder()(&map, type, rank, const_cast<void*>(ptr), dims, strides, box, estr,
@@ -802,7 +803,8 @@ void launch_split(const MxGemmDesc& d, const MxArgs& args, cudaStream_t stream) 
   auto kernel = mx_gemm_split_kernel<T, FMT, MT>;
   static PerDeviceOnce once, asked;
   raise_smem_limit(once, kernel, S::SMEM_BYTES);
-  const unsigned tiles_n = static_cast<unsigned>((d.N + 127) / 128), tiles_m = static_cast<unsigned>((d.M + MT - 1) / MT);
+  const unsigned tiles_n = static_cast<unsigned>((d.N + 127) / 128);
+  const unsigned tiles_m = static_cast<unsigned>((d.M + MT - 1) / MT);
   cudaLaunchConfig_t cfg{};
   cfg.blockDim = dim3(192);
   cfg.dynamicSmemBytes = S::SMEM_BYTES;
@@ -847,7 +849,8 @@ void launch(const MxGemmDesc& d, cudaStream_t stream) {
   const long pairs = static_cast<long>((d.M + 255) / 256) * ((d.N + 255) / 256);
   if (d.M <= 32) return launch_split<T, FMT, 32>(d, args, stream);
   if (2 * tiles <= sms && args.num_kb > 1) return launch_split<T, FMT, 128>(d, args, stream);
-  if ((pairs + sms / 2 - 1) / (sms / 2) <= (tiles + sms - 1) / sms) return launch_tiles<T, FMT, 256, 2>(d, args, stream);
+  if ((pairs + sms / 2 - 1) / (sms / 2) <= (tiles + sms - 1) / sms)
+    return launch_tiles<T, FMT, 256, 2>(d, args, stream);
   launch_tiles<T, FMT, 128, 1>(d, args, stream);
 }
 

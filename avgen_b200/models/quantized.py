@@ -97,8 +97,10 @@ def quantize_model(model: nn.Module, fmt: str = "mxfp8") -> int:
         for block in blocks.values():
             att, ff, ca = block.attention, block.feed_forward, block.cross_attention
             up = (ff.gate_proj, ff.up_proj) if hasattr(ff, "gate_proj") else (ff.up_proj,)
-            cross = {} if ca is None else {"cross_q": _pack(fmt, ca.q_proj), "cross_kv": _pack(fmt, ca.k_proj, ca.v_proj),
-                                           "cross_out": _pack(fmt, ca.out_proj)}
+            cross = {}
+            if ca is not None:
+                cross = {"cross_q": _pack(fmt, ca.q_proj), "cross_kv": _pack(fmt, ca.k_proj, ca.v_proj),
+                         "cross_out": _pack(fmt, ca.out_proj)}
             block.quantized = QuantizedBlock(fmt, qkv=_pack(fmt, att.q_proj, att.k_proj, att.v_proj),
                                              out=_pack(fmt, att.out_proj), up=_pack(fmt, *up),
                                              down=_pack(fmt, ff.down_proj), **cross)
@@ -166,11 +168,12 @@ def quantized_block_forward(block: nn.Module, hidden: torch.Tensor, combined: to
     """One block on its packed weights; arguments as the fused block takes them (``combined``:
     modulation rows with the block's table added, picked per token by ``mod_index``)."""
     if torch.is_grad_enabled():
-        raise RuntimeError("a quantised block has no gradient; run it under torch.no_grad() or call restore_model first")
+        raise RuntimeError("a quantised block has no gradient; run it under torch.no_grad() or call restore_model "
+                           "first")
     p = block.quantized
     if p.qkv.device != hidden.device:
-        raise RuntimeError(f"packed weights are on {p.qkv.device}, the input on {hidden.device}: call quantize_model after "
-                           "moving the model")
+        raise RuntimeError(f"packed weights are on {p.qkv.device}, the input on {hidden.device}: call quantize_model "
+                           "after moving the model")
     b, length, w = hidden.shape
     fmt, eps = p.fmt, block.attention_norm.eps or 1e-6
     groups, per = None, length

@@ -289,8 +289,8 @@ def _dequantize_reference(t: MXTensor) -> torch.Tensor:
     return v if t.global_scale is None else v * t.global_scale
 
 
-def _add_rmsnorm_reference(x, update, weight, scale, shift, gate, rows_per_batch, groups, eps, fmt,  # noqa: ANN001, ANN202
-                           global_scale):
+def _add_rmsnorm_reference(x, update, weight, scale, shift, gate, rows_per_batch, groups, eps,  # noqa: ANN001, ANN202
+                           fmt, global_scale):
     cols = x.shape[-1]
     v = x.reshape(-1, cols).float()
     rows = torch.arange(v.shape[0]) // max(1, rows_per_batch) if groups is None else groups.long()

@@ -36,7 +36,8 @@ def test_quantize_rounds_to_the_nearest_value_of_its_scale(fmt: str, shape: tupl
 @pytest.mark.parametrize("fmt", ["mxfp8", "mxfp4"])
 def test_power_scales_are_the_smallest_that_saturate_nothing(fmt: str) -> None:
     top = oracle.TOP[fmt]
-    amax = torch.tensor([0.0, 1e-45, 2.0 ** -130, 2.0 ** -126, 1.0, top, top * 1.0001, top / 2, 3.3e38, 7.0, 6.0, 449.0])
+    amax = torch.tensor([0.0, 1e-45, 2.0 ** -130, 2.0 ** -126, 1.0, top, top * 1.0001, top / 2, 3.3e38, 7.0, 6.0,
+                         449.0])
     x = torch.zeros(len(amax), 32)
     x[:, 5] = -amax
     t = mx.quantize(x, fmt)
@@ -98,7 +99,8 @@ def test_add_rmsnorm_reference_matches_its_formula() -> None:
 
 def test_matmul_reference() -> None:
     gen = torch.Generator().manual_seed(5)
-    a, b = mx.quantize(torch.randn(3, 50, generator=gen), "mxfp4"), mx.quantize(torch.randn(7, 50, generator=gen), "mxfp4")
+    a = mx.quantize(torch.randn(3, 50, generator=gen), "mxfp4")
+    b = mx.quantize(torch.randn(7, 50, generator=gen), "mxfp4")
     out = mx.matmul(a, b, bias=torch.arange(7.0), out_dtype=torch.float32)
     want = oracle.decode(a) @ oracle.decode(b).t() + torch.arange(7.0)
     assert (out.double() - want).abs().max() < 1e-5 * (1 + want.abs().max())
