@@ -16,7 +16,9 @@ projections and the output head stay in bf16: they are small, and precision-sens
 
 The blocks keep their own weights (checkpoints, adapters and training are not touched);
 :func:`restore_model` drops the packed ones. A quantised block has no gradient and refuses
-to run while gradients are recorded. On the CPU the same code runs the operators' PyTorch
+to run while gradients are recorded, and under context or head-parallel tensor parallelism,
+which leave a rank with part of the tokens or heads, whether they were applied before or
+after packing. On the CPU the same code runs the operators' PyTorch
 restatement. The reference framework has no counterpart: its only low-precision option is
 a third-party package's fp8 training (avgen/parallel/precision.py:212-284).
 """
@@ -55,14 +57,25 @@ class QuantizedBlock:
         return sum(p.nbytes for p in parts if p is not None)
 
 
+def _split_by(block: nn.Module) -> str | None:
+    """The parallelism that spreads the block's heads or tokens over ranks, if any."""
+    if block.attention_impl is not None or block.attention.cp_mesh is not None:
+        return "context parallelism"
+    parts = (block, block.attention, block.cross_attention, block.feed_forward)
+    if any(getattr(m, "tp", None) is not None for m in parts):
+        return "head-parallel tensor parallelism"
+    return None
+
+
 def _check(block: nn.Module, name: str) -> None:
     from torch.distributed.tensor import DTensor
 
     linears = {n: m for n, m in block.named_modules() if isinstance(m, nn.Linear)}
-    if any(isinstance(m.weight, DTensor) for m in linears.values()) or getattr(block, "tp", None) is not None:
-        raise ValueError(f"{name}: sharded weights cannot be quantised; quantise before parallelising or gather first")
-    if block.attention_impl is not None or block.attention.cp_mesh is not None:
-        raise ValueError(f"{name}: quantised blocks attend locally, without context parallelism")
+    split = _split_by(block)
+    if split is not None:
+        raise ValueError(f"{name}: a quantised block takes whole heads and sequences, it does not run under {split}")
+    if any(isinstance(m.weight, DTensor) for m in linears.values()):
+        raise ValueError(f"{name}: sharded weights cannot be quantised; quantise before sharding or gather first")
     biased = [n for n, m in linears.items() if m.bias is not None]
     if biased:
         raise ValueError(f"{name}: quantised linears have no bias; found {', '.join(biased)}")
@@ -170,6 +183,9 @@ def quantized_block_forward(block: nn.Module, hidden: torch.Tensor, combined: to
     if torch.is_grad_enabled():
         raise RuntimeError("a quantised block has no gradient; run it under torch.no_grad() or call restore_model "
                            "first")
+    split = _split_by(block)
+    if split is not None:  # set after packing: this rank's share alone would be attended to
+        raise RuntimeError(f"a quantised block does not run under {split}; call restore_model first")
     p = block.quantized
     if p.qkv.device != hidden.device:
         raise RuntimeError(f"packed weights are on {p.qkv.device}, the input on {hidden.device}: call quantize_model "

@@ -137,6 +137,49 @@ def test_state_and_refusals() -> None:
         quantize_model(nn.ModuleList([_block(), biased]), "mxfp8")
 
 
+def _parallelise(block: DiTBlock, where: str) -> None:
+    if where == "cp fused":
+        block.attention_impl = object()
+    elif where == "cp eager":
+        block.attention.cp_mesh = object()
+    else:
+        {"tp": block, "tp attention": block.attention, "tp cross": block.cross_attention,
+         "tp mlp": block.feed_forward}[where].tp = object()
+
+
+@pytest.mark.parametrize("where,kind", [("cp fused", "context"), ("cp eager", "context"), ("tp", "tensor"),
+                                        ("tp attention", "tensor"), ("tp cross", "tensor"), ("tp mlp", "tensor")])
+def test_parallelism_applied_after_packing_is_refused(where: str, kind: str) -> None:
+    """A block that holds part of the tokens or heads must not attend to that part alone."""
+    block = _block()
+    hidden, kwargs = _inputs("sample")
+    quantize_model(block, "mxfp8")
+    _parallelise(block, where)
+    with torch.no_grad(), pytest.raises(RuntimeError, match=f"{kind} parallelism"):
+        block(hidden, **kwargs)
+    restore_model(block)
+    with pytest.raises(ValueError, match=f"{kind} parallelism"):
+        quantize_model(block, "mxfp8")
+
+
+def test_context_parallelism_over_packed_blocks_is_refused() -> None:
+    from avgen_b200.parallel.context import apply_context_parallel
+
+    class Mesh:  # what context parallelism asks of a mesh before its first collective
+        def size(self) -> int:
+            return 2
+
+        def get_group(self) -> None:
+            return None
+
+    model = nn.ModuleList([_block()])
+    hidden, kwargs = _inputs("sample")
+    quantize_model(model, "mxfp8")
+    apply_context_parallel(model, Mesh(), ring=False)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="context parallelism"):
+        model[0](hidden, **kwargs)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("fmt", mx.FORMATS)
 @pytest.mark.parametrize("ffn,form", [("swiglu", "sample"), ("gelu", "grouped"), ("swiglu", "token")])
