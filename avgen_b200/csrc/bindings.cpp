@@ -1025,7 +1025,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> mx_add_rmsnorm(const at::Tensor& 
   d.W = static_cast<int>(rows.size(1));
   d.eps = static_cast<float>(eps);
   d.x = rows.data_ptr();
-  TORCH_CHECK(d.rows < (1L << 31) - 256, "add_rmsnorm: too many rows");
+  TORCH_CHECK(d.rows <= mx_norm_max_rows(d.device), "add_rmsnorm: at most ", mx_norm_max_rows(d.device), " rows, got ",
+              d.rows);
   d.ldx = rows.stride(0);
   at::Tensor u, out = x;
   if (has(update)) {

@@ -442,6 +442,7 @@ struct MxNormDesc {
   const float* g = nullptr;
 };
 constexpr int kMxNormMaxCols = 65536;  // a row stays in one CTA's registers
+long mx_norm_max_rows(int device);     // above it the kernel's row numbers would overflow
 void mx_add_rmsnorm_launch(const MxNormDesc& d, cudaStream_t stream);
 
 // out[M, N] = A[M, K] . B[N, K]^T (+ bias), both operands in format `fmt`.

@@ -17,6 +17,7 @@
 //   norm       to mxfp8 192 (6.1), with two modulation levels 221 (5.3); 16387 x 5120 99
 //              (5.9); 20000 x 5001, whose rows are not aligned, 227 (3.1)
 #include <algorithm>
+#include <limits>
 
 #include "include/host_utils.h"
 #include "include/launchers.h"
@@ -818,6 +819,8 @@ void dequantize(const MxDequantDesc& d, cudaStream_t stream) {
   else dequantize_as<T, FMT, false>(d, p, stream);
 }
 
+constexpr int kNormWarpsPerSm = 64;  // of a launch: the most rows one step of the norm's loop passes over, per SM
+
 template <typename T, int FMT, int CHUNKS, bool WARP_ROWS, bool ALIGNED>
 void add_rmsnorm_as(const MxNormDesc& d, const PackedRows& p, int warps, cudaStream_t stream) {
   auto kernel = d.gate != nullptr || d.scale != nullptr || d.shift != nullptr
@@ -825,7 +828,7 @@ void add_rmsnorm_as(const MxNormDesc& d, const PackedRows& p, int warps, cudaStr
                     : mx_add_rmsnorm_kernel<T, FMT, CHUNKS, WARP_ROWS, ALIGNED, false>;
   const long padded = (d.rows + 127) / 128 * 128;
   const long units = WARP_ROWS ? (padded + warps - 1) / warps : padded;
-  const long ctas = static_cast<long>(std::max(1, 64 / warps)) * num_sms(d.device);
+  const long ctas = static_cast<long>(std::max(1, kNormWarpsPerSm / warps)) * num_sms(d.device);
   const int smem = ALIGNED ? 0 : warps * kNormSpan * 4;  // at most 32 KB
   kernel<<<static_cast<unsigned>(std::min(units, ctas)), 32 * warps, smem, stream>>>(d, p);
   AVGEN_CUDA_CHECK(cudaGetLastError());
@@ -877,6 +880,12 @@ int mx_quantize_parts(const MxQuantDesc& d) {
   // CTAs of the measuring pass: up to eight for every SM, a row per warp at least
   const long blocks = std::min<long>((d.rows + 7) / 8, std::max<long>(1, 8L * num_sms(d.device) / segments));
   return static_cast<int>(blocks * segments);
+}
+
+// The norm counts rows in 32 signed bits; the last row of the last 128-row group plus one
+// step has to stay within them.
+long mx_norm_max_rows(int device) {
+  return std::numeric_limits<int>::max() - 127L - static_cast<long>(kNormWarpsPerSm) * num_sms(device);
 }
 
 void mx_quantize_launch(const MxQuantDesc& d, cudaStream_t stream) { AVGEN_MX_DISPATCH(quantize, d, stream); }

@@ -190,6 +190,16 @@ def test_add_rmsnorm_edges() -> None:
     assert (mx.dequantize(t4, torch.float32) - back[4]).abs().max() < 0.5
 
 
+@pytest.mark.parametrize("rows", [2 ** 31 - 257, 2 ** 31 - 9000])
+def test_add_rmsnorm_refuses_rows_past_its_row_numbers(rows: int) -> None:
+    """Rows are counted in 32 signed bits: the last row plus one step of the loop (up to 64
+    rows an SM) has to fit. One column, repeated without memory of its own."""
+    most = 2 ** 31 - 128 - 64 * torch.cuda.get_device_properties(0).multi_processor_count
+    x = torch.ones(1, 1, device=DEV).expand(rows, 1)
+    with pytest.raises(RuntimeError, match=f"at most {most} rows, got {rows}"):
+        mx.add_rmsnorm_mod(x, None, None, fmt="mxfp4")
+
+
 # ----------------------------------------------------------------------------- product
 PRODUCTS = [(1, 1, 1), (1, 8, 32), (2, 130, 65), (128, 128, 256), (129, 127, 96), (200, 300, 1000), (257, 513, 2570),
             (1, 2560, 2560), (16, 640, 4096), (33, 1024, 160), (64, 200, 13824), (640, 384, 129), (1000, 2568, 512),
