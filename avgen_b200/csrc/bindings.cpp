@@ -933,6 +933,8 @@ const float* mx_global(const OptT& g, const at::Tensor& like, const char* name) 
 long check_packed(const at::Tensor& codes, const at::Tensor& scales, int fmt, long cols, const char* name) {
   TORCH_CHECK(fmt >= kMxFp8 && fmt <= kNvFp4, name, ": unknown format ", fmt);
   TORCH_CHECK(cols > 0, name, ": needs at least one column");
+  TORCH_CHECK(codes.dim() != 2 || codes.size(0) <= kMxMaxRows, name, ": at most ", kMxMaxRows, " rows, got ",
+              codes.size(0));
   check_cuda(codes, name);
   TORCH_CHECK(codes.scalar_type() == at::kByte && codes.dim() == 2 && codes.is_contiguous() &&
                   codes.size(1) == mx_row_bytes(fmt, cols),

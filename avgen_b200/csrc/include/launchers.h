@@ -382,6 +382,7 @@ void mt_adamw_launch(const MTChunk* chunks, int nchunks, const MTTensor* tensors
 // Block-scaled formats (microscale.cu, mx_gemm.cu; the formats themselves are in
 // microscale.cuh). `fmt` is an MxFormat; `dtype` is the type of the plain tensor.
 enum MxDType : int { kMxBf16 = 0, kMxFp16 = 1, kMxFp32 = 2 };
+constexpr long kMxMaxRows = 1L << 32;  // of a packed tensor: kernels place a row's scales by 32-bit row numbers
 
 struct MxQuantDesc {
   int device = 0;

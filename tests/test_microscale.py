@@ -149,6 +149,19 @@ def test_extension_error_messages_format_numbers() -> None:
     assert done.returncode == 0 and "unknown format 77" in done.stdout
 
 
+def test_packed_rows_past_32_bits_are_refused() -> None:
+    """A row's scales are found by its number in 32 bits: past them it would get another row's."""
+    from avgen_b200.ops import _ext
+
+    if not _ext.available():
+        pytest.skip("extension not built")
+    rows = 2 ** 32 + 1
+    codes = torch.zeros(1, 16, dtype=torch.uint8).expand(rows, 16)
+    scales = torch.zeros(1, dtype=torch.uint8).expand(-(-rows // 128) * 512)
+    with pytest.raises(RuntimeError, match=f"at most {2 ** 32} rows, got {rows}"):
+        _ext.load().mx_dequantize(codes, scales, 1, 1, None, torch.float32)
+
+
 def test_packed_size() -> None:
     t = mx.quantize(torch.zeros(256, 512), "nvfp4")
     assert t.nbytes == 256 * 512 // 2 + 256 * 512 // 16 + 4
