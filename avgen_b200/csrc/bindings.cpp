@@ -8,6 +8,8 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <limits>
+
 #include "include/host_utils.h"
 #include "include/launchers.h"
 #include "include/microscale.cuh"
@@ -1068,8 +1070,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> mx_add_rmsnorm(const at::Tensor& 
   if (mod_rows >= 0) {
     d.groups = groups_or_null(groups, d.rows, "add_rmsnorm");
     TORCH_CHECK(d.groups == nullptr || groups->device() == x.device(), "add_rmsnorm: groups must be on x's device");
-    d.num_groups = static_cast<int>(mod_rows);
-    TORCH_CHECK(d.groups != nullptr || mod_rows * d.rows_per_batch >= d.rows,
+    d.num_groups = static_cast<int>(std::min<long>(mod_rows, std::numeric_limits<int>::max()));  // groups are int32
+    TORCH_CHECK(d.groups != nullptr || (d.rows - 1) / d.rows_per_batch < mod_rows,
                 "add_rmsnorm: modulation rows do not cover x");
   }
   auto [codes, scales] = mx_empty_packed(d.fmt, d.rows, d.W, x.device());

@@ -200,6 +200,16 @@ def test_add_rmsnorm_refuses_rows_past_its_row_numbers(rows: int) -> None:
         mx.add_rmsnorm_mod(x, None, None, fmt="mxfp4")
 
 
+def test_add_rmsnorm_picks_from_a_modulation_table_of_2_to_the_31_rows() -> None:
+    shift = torch.zeros(2 ** 31, 1, device=DEV)
+    shift[2 ** 31 - 1], shift[5] = 2.0, 4.0
+    groups = torch.tensor([5, 2 ** 31 - 1, 6], dtype=torch.int32, device=DEV)
+    _, t = mx.add_rmsnorm_mod(torch.zeros(3, 1, device=DEV), None, None, None, shift, groups=groups)
+    assert mx.dequantize(t, torch.float32).flatten().tolist() == [4.0, 2.0, 0.0]
+    _, t = mx.add_rmsnorm_mod(torch.zeros(3, 1, device=DEV), None, None, None, shift[:8], rows_per_batch=2 ** 62)
+    assert not mx.dequantize(t).any()
+
+
 # ----------------------------------------------------------------------------- product
 PRODUCTS = [(1, 1, 1), (1, 8, 32), (2, 130, 65), (128, 128, 256), (129, 127, 96), (200, 300, 1000), (257, 513, 2570),
             (1, 2560, 2560), (16, 640, 4096), (33, 1024, 160), (64, 200, 13824), (640, 384, 129), (1000, 2568, 512),
