@@ -1061,10 +1061,15 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> mx_add_rmsnorm(const at::Tensor& 
   d.scale = mod(scale, "scale");
   d.shift = mod(shift, "shift");
   d.gate = mod(gate, "gate");
-  if (d.scale != nullptr) d.mod_stride = scale->stride(0);
-  if (d.shift != nullptr) {
-    TORCH_CHECK(d.scale == nullptr || shift->stride(0) == d.mod_stride, "add_rmsnorm: scale and shift strides differ");
-    d.mod_stride = shift->stride(0);
+  at::Tensor even_scale, even_shift;
+  if (d.scale != nullptr && d.shift != nullptr && scale->stride(0) != shift->stride(0)) {
+    even_scale = scale->contiguous();  // the kernel takes one stride for both
+    even_shift = shift->contiguous();
+    d.scale = even_scale.data_ptr<float>();
+    d.shift = even_shift.data_ptr<float>();
+    d.mod_stride = d.W;
+  } else if (d.scale != nullptr || d.shift != nullptr) {
+    d.mod_stride = d.scale != nullptr ? scale->stride(0) : shift->stride(0);
   }
   if (d.gate != nullptr) d.gate_stride = gate->stride(0);
   if (mod_rows >= 0) {

@@ -177,6 +177,18 @@ def test_add_rmsnorm_rows_per_batch_and_strides() -> None:
     assert torch.equal(a, b.view(64, 640)) and torch.equal(ta.codes, tb.codes) and torch.equal(ta.scales, tb.scales)
 
 
+@pytest.mark.parametrize("rows", [1, 4])
+def test_add_rmsnorm_scale_and_shift_of_different_strides(rows: int) -> None:
+    wide, x = torch.randn(rows, 6, 640, device=DEV), torch.randn(16 * rows, 640, device=DEV).bfloat16()
+    plain = wide[:, 0].clone()
+    once = torch.randn(640, device=DEV).expand(rows, 640)
+    for scale, shift in ((wide[:, 1], plain), (plain, wide[:, 1]), (once, plain), (wide[:, 1], once)):
+        _, got = mx.add_rmsnorm_mod(x, None, None, scale, shift, rows_per_batch=16)
+        _, want = mx.add_rmsnorm_mod(x, None, None, scale.clone(memory_format=torch.contiguous_format),
+                                     shift.clone(memory_format=torch.contiguous_format), rows_per_batch=16)
+        assert torch.equal(got.codes, want.codes) and torch.equal(got.scales, want.scales)
+
+
 def test_add_rmsnorm_edges() -> None:
     x = torch.zeros(5, 96, device=DEV)
     x[1], x[2, 4], x[3, 90] = 1e30, float("nan"), float("inf")
