@@ -1075,7 +1075,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> mx_add_rmsnorm(const at::Tensor& 
   if (mod_rows >= 0) {
     d.groups = groups_or_null(groups, d.rows, "add_rmsnorm");
     TORCH_CHECK(d.groups == nullptr || groups->device() == x.device(), "add_rmsnorm: groups must be on x's device");
-    d.num_groups = static_cast<int>(std::min<long>(mod_rows, std::numeric_limits<int>::max()));  // groups are int32
+    d.last_mod_row = static_cast<int>(std::min<long>(mod_rows - 1, std::numeric_limits<int>::max()));  // groups are int32
     TORCH_CHECK(d.groups != nullptr || (d.rows - 1) / d.rows_per_batch < mod_rows,
                 "add_rmsnorm: modulation rows do not cover x");
   }

@@ -436,7 +436,7 @@ struct MxNormDesc {
   const float* gate = nullptr;
   long gate_stride = 0;
   const int* groups = nullptr;
-  int num_groups = 0;
+  int last_mod_row = -1;  // of scale, shift and gate; groups beyond it take it
   long rows_per_batch = 1;
   uint8_t* codes = nullptr;
   uint8_t* scales = nullptr;

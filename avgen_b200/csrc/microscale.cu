@@ -636,7 +636,9 @@ __global__ void __launch_bounds__(CHUNKS == 8 ? 1024 : WARP_ROWS ? 128 : 512,
   Chunk<T, ALIGNED> rx[CHUNKS], ru[CHUNKS];
   int next_b = 0;
   auto request = [&](int at) {
-    if (d.num_groups > 0) next_b = static_cast<int>(mod_row(d.groups, d.num_groups, at, d.rows_per_batch));
+    if (d.last_mod_row >= 0)
+      next_b = d.groups != nullptr ? max(0, min(__ldg(d.groups + at), d.last_mod_row))
+                                   : static_cast<int>(at / d.rows_per_batch);
     const NormRow<T, ALIGNED> x(reinterpret_cast<const T*>(d.x), at * d.ldx, 0.f);
     const NormRow<T, ALIGNED> u(reinterpret_cast<const T*>(d.update), at * d.ldu, 0.f);
 #pragma unroll
