@@ -1,10 +1,10 @@
 // Block-scaled tcgen05 product for sm_100a.
 //
-//   D[M, N] = alpha * (A . B^T) (+ bias),  A [M, K], B [N, K] in mxfp8, mxfp4 or nvfp4
+//   D[M, N] = (A . B^T) * g_a * g_b (+ bias),  A [M, K], B [N, K] in mxfp8, mxfp4 or nvfp4
 //
 // The tensor cores multiply each block's products by both block scales while they
 // accumulate in fp32 (kind::mxf8f6f4 / mxf4 / mxf4nvf4 with .block_scale), so the
-// operands stay packed all the way; alpha = g_a * g_b is nvfp4's pair of tensor scales.
+// operands stay packed all the way; g_a and g_b are nvfp4's tensor scales, else 1.
 //
 // Structure (persistent over output tiles; CTAS = 2 pairs the two SMs of a TPC on one
 // 256 x 256 tile, CTAS = 1 gives each SM a 128 x 128 tile):
@@ -31,6 +31,7 @@
 //   16384 x 2560 x 10240 mxfp4   165 us, 5.2 PFLOP/s (6.1)
 //   32768 x 5120 x 5120 mxfp8    686 us, 2.5 PFLOP/s (2.9)
 #include <algorithm>
+#include <cfloat>
 
 #include "include/host_utils.h"
 #include "include/launchers.h"
@@ -274,6 +275,24 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, err, code));
 }
 
+// nvfp4's two tensor scales as factors that a sum takes one after the other. Their product
+// alone may leave fp32's range where the result does not (sums reach 2688^2 * K): then the
+// larger one goes first if it is too small, the smaller one if it is too large.
+struct TensorScales {
+  float first, last;
+
+  __device__ __forceinline__ explicit TensorScales(const MxArgs& args) {
+    const float a = args.a_g != nullptr ? *args.a_g : 1.f, b = args.b_g != nullptr ? *args.b_g : 1.f;
+    const float both = a * b;
+    const bool swap = (fabsf(both) < 1.f) != (fabsf(a) > fabsf(b));
+    first = swap ? b : a;
+    last = swap ? a : b;
+    if (fabsf(both) >= FLT_MIN && fabsf(both) <= FLT_MAX) first = 1.f, last = both;
+  }
+  __device__ __forceinline__ float operator()(float sum) const { return sum * first * last; }
+  __device__ __forceinline__ float operator()(float sum, float bias) const { return fmaf(sum * first, last, bias); }
+};
+
 // After an abort: copies still in flight land well within a millisecond.
 __device__ __forceinline__ void let_copies_land() {
   const uint64_t t0 = globaltimer();
@@ -459,7 +478,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr int BOX = 128 / static_cast<int>(sizeof(T));  // columns of a store box
     const int q = warp & 3, half = (warp - 2) >> 2;
     uint8_t* box = smem_out + (warp - 2) * kBoxBytes;
-    const float alpha = (args.a_g != nullptr ? *args.a_g : 1.f) * (args.b_g != nullptr ? *args.b_g : 1.f);
+    const TensorScales scaled(args);
     uint32_t release[2];
     for (int b = 0; b < 2; ++b)
       release[b] = CTAS == 2 ? map_to_rank(smem_u32(&tempty[b]), 0) : smem_u32(&tempty[b]);
@@ -499,7 +518,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (row0 >= args.M || col0 >= args.N) continue;
         float v[64];
 #pragma unroll
-        for (int j = 0; j < 64; ++j) v[j] = __uint_as_float(r[j / 32][j % 32]) * alpha;
+        for (int j = 0; j < 64; ++j) v[j] = scaled(__uint_as_float(r[j / 32][j % 32]));
         if (args.bias != nullptr) {
 #pragma unroll
           for (int j = 0; j < 64; ++j) v[j] += col0 + j < args.N ? __ldg(args.bias + col0 + j) : 0.f;
@@ -634,7 +653,7 @@ __global__ void __launch_bounds__(192, 1)
     const int q = warp & 3;
     const int lane_n = q * 32 + lane, n = n0 + lane_n;
     const int rows = min(MT, args.M - m0);
-    const float alpha = (args.a_g != nullptr ? *args.a_g : 1.f) * (args.b_g != nullptr ? *args.b_g : 1.f);
+    const TensorScales scaled(args);
     const float bias = args.bias != nullptr && n < args.N ? args.bias[n] : 0.f;
     float* partial = reinterpret_cast<float*>(smem);  // [row][128 weight rows]: every staged block has been multiplied
 #pragma unroll
@@ -651,7 +670,7 @@ __global__ void __launch_bounds__(192, 1)
           partial[m * 128 + lane_n] = __uint_as_float(r[i]);
         else if (n < args.N)
           reinterpret_cast<T*>(args.out)[static_cast<long>(m0 + m) * args.N + n] =
-              from_float<T>(fmaf(__uint_as_float(r[i]), alpha, bias));
+              from_float<T>(scaled(__uint_as_float(r[i]), bias));
       }
     }
   }
@@ -661,7 +680,7 @@ __global__ void __launch_bounds__(192, 1)
     if (warp >= 2) {  // a warp per row, four columns per lane, every CTA's part requested before the first is added
       const int n = n0 + 4 * lane;
       const int rows = min(MT, args.M - m0);
-      const float alpha = (args.a_g != nullptr ? *args.a_g : 1.f) * (args.b_g != nullptr ? *args.b_g : 1.f);
+      const TensorScales scaled(args);
       float bias[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) bias[j] = args.bias != nullptr && n + j < args.N ? args.bias[n + j] : 0.f;
@@ -686,8 +705,8 @@ __global__ void __launch_bounds__(192, 1)
         for (int s = 1; s < kMaxSplits; ++s)
           sum.x += part[s].x, sum.y += part[s].y, sum.z += part[s].z, sum.w += part[s].w;
         T* out = reinterpret_cast<T*>(args.out) + static_cast<long>(m0 + m) * args.N + n;
-        alignas(16) T v[4] = {from_float<T>(fmaf(sum.x, alpha, bias[0])), from_float<T>(fmaf(sum.y, alpha, bias[1])),
-                              from_float<T>(fmaf(sum.z, alpha, bias[2])), from_float<T>(fmaf(sum.w, alpha, bias[3]))};
+        alignas(16) T v[4] = {from_float<T>(scaled(sum.x, bias[0])), from_float<T>(scaled(sum.y, bias[1])),
+                              from_float<T>(scaled(sum.z, bias[2])), from_float<T>(scaled(sum.w, bias[3]))};
         if (whole) {  // rows on 4 values
           if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(v);
           else *reinterpret_cast<uint4*>(out) = *reinterpret_cast<const uint4*>(v);

@@ -293,6 +293,31 @@ def test_matmul_non_finite_rows_stay_in_their_rows(fmt: str) -> None:
     assert torch.equal(torch.isnan(got), bad)
 
 
+# one row, few rows, one tile a CTA and one tile a CTA pair
+SCALED = [(1, 64, 13824), (3, 130, 64), (100, 200, 1024), (300, 20000, 520), (2400, 2100, 160)]
+
+
+@pytest.mark.parametrize("shape", SCALED)
+@pytest.mark.parametrize("sizes", [(1e-18, 1e-18), (3e-19, 1e-20), (1e-28, 1e-9), (1e15, 1e17), (1e-30, 1e30)])
+def test_matmul_of_operands_of_any_size(shape: tuple[int, int, int], sizes: tuple[float, float]) -> None:
+    """The tensor scales' product leaves fp32's range, or nearly, where the results do not."""
+    m, n, k = shape
+    a = mx.quantize((_rows(m, k, m + k) * sizes[0]).to(DEV), "nvfp4")
+    b = mx.quantize((_rows(n, k, n) * sizes[1]).to(DEV), "nvfp4")
+    _check_product(a, b, None, torch.float32)
+
+
+@pytest.mark.parametrize("shape", SCALED)
+def test_matmul_of_tensor_scales_whose_product_overflows(shape: tuple[int, int, int]) -> None:
+    m, n, k = shape
+    g, size = torch.tensor([2.0 ** 66], device=DEV), 6 * 2.0 ** -9 * 2.0 ** 66  # code 6, the smallest block scale
+    x, w = torch.zeros(m, k, device=DEV), torch.full((n, k), size, device=DEV)
+    x[::2, :16] = size
+    got = mx.matmul(mx.quantize(x, "nvfp4", global_scale=g), mx.quantize(w, "nvfp4", global_scale=g),
+                    out_dtype=torch.float32)
+    assert (got[::2] == 16 * size ** 2).all() and not got[1::2].any()
+
+
 @pytest.mark.parametrize("fmt", mx.FORMATS)
 @pytest.mark.parametrize("m", [1, 40, 300])
 def test_matmul_repeats_bitwise(fmt: str, m: int) -> None:
