@@ -35,6 +35,8 @@ from avgen_b200.models.attention import attention
 from avgen_b200.models.rope import apply_rotary
 from avgen_b200.ops import microscale as mx
 
+_NVFP4_RANGE = 6.0 * 448.0  # largest e2m1 times largest e4m3
+
 __all__ = ["QuantizedBlock", "quantize_model", "quantized_block_forward", "restore_model"]
 
 
@@ -50,6 +52,9 @@ class QuantizedBlock:
     cross_q: mx.MXTensor | None = None
     cross_kv: mx.MXTensor | None = None
     cross_out: mx.MXTensor | None = None
+    # nvfp4: tensor scales [1] that hold the whole range of an un-modulated norm's output
+    # (self-attention's, cross-attention's and the MLP's); None for the other formats
+    norm_scales: tuple[torch.Tensor, torch.Tensor | None, torch.Tensor] | None = None
 
     @property
     def nbytes(self) -> int:
@@ -91,6 +96,27 @@ def _weight(layer: nn.Linear) -> torch.Tensor:
     return (adapted() if callable(adapted) else layer.weight).detach()
 
 
+def _norm_scale(norm: nn.Module, width: int, device: torch.device) -> torch.Tensor:
+    """The nvfp4 tensor scale of a norm's output before modulation: no normalised value is
+    above sqrt(width), and the largest a tensor scale g can hold is 2688 g."""
+    w = _norm_weight(norm)
+    gain = torch.ones(1, device=device) if w is None else w.abs().amax().reshape(1)
+    return (gain * (math.sqrt(width) / _NVFP4_RANGE)).clamp(min=2.0 ** -100)
+
+
+def _modulated_scales(combined: torch.Tensor, p: QuantizedBlock) -> tuple[torch.Tensor, torch.Tensor]:
+    """Tensor scales of the two modulated norms, from the largest shift and 1 + |scale| of the
+    call: |y| <= 2688 g (1 + |scale|) + |shift|, so nothing saturates, and blocks down to
+    1 / 28000 of that bound keep normal scales. A modulation that is not finite (its rows are
+    NaN in any case) counts as 2, so that other rows stay what they are."""
+    if len(combined) == 0:
+        return p.norm_scales[0], p.norm_scales[2]
+    peak = torch.linalg.vector_norm(combined, float("inf"), dim=(0, 2)).nan_to_num(nan=2.0, posinf=2.0)  # [6]
+    own = torch.cat((p.norm_scales[0], p.norm_scales[2]))
+    g = torch.addcmul(own, own, peak[1::3]).add_(peak[0::3], alpha=1.0 / _NVFP4_RANGE)
+    return g[:1], g[1:]
+
+
 def _pack(fmt: str, *layers: nn.Linear) -> mx.MXTensor:
     w = [_weight(layer) for layer in layers]
     return mx.quantize(w[0] if len(w) == 1 else torch.cat(w, 0), fmt)
@@ -110,13 +136,18 @@ def quantize_model(model: nn.Module, fmt: str = "mxfp8") -> int:
         for block in blocks.values():
             att, ff, ca = block.attention, block.feed_forward, block.cross_attention
             up = (ff.gate_proj, ff.up_proj) if hasattr(ff, "gate_proj") else (ff.up_proj,)
-            cross = {}
+            more = {}
             if ca is not None:
-                cross = {"cross_q": _pack(fmt, ca.q_proj), "cross_kv": _pack(fmt, ca.k_proj, ca.v_proj),
-                         "cross_out": _pack(fmt, ca.out_proj)}
+                more = {"cross_q": _pack(fmt, ca.q_proj), "cross_kv": _pack(fmt, ca.k_proj, ca.v_proj),
+                        "cross_out": _pack(fmt, ca.out_proj)}
+            if fmt == "nvfp4":
+                device = att.q_proj.weight.device
+                more["norm_scales"] = (_norm_scale(block.attention_norm, block.width, device),
+                                       _norm_scale(block.cross_norm, block.width, device) if ca is not None else None,
+                                       _norm_scale(block.ffn_norm, block.width, device))
             block.quantized = QuantizedBlock(fmt, qkv=_pack(fmt, att.q_proj, att.k_proj, att.v_proj),
                                              out=_pack(fmt, att.out_proj), up=_pack(fmt, *up),
-                                             down=_pack(fmt, ff.down_proj), **cross)
+                                             down=_pack(fmt, ff.down_proj), **more)
     return len(blocks)
 
 
@@ -198,24 +229,29 @@ def quantized_block_forward(block: nn.Module, hidden: torch.Tensor, combined: to
     elif combined.ndim == 4:
         combined, per = combined.reshape(b * length, *combined.shape[2:]), 1
     rows = {"rows_per_batch": per, "groups": groups}
-    shift_a, scale_a, gate_a, shift_f, scale_f, gate_f = combined.float().contiguous().unbind(1)
+    combined = combined.float().contiguous()
+    shift_a, scale_a, gate_a, shift_f, scale_f, gate_f = combined.unbind(1)
+    g_a = g_c = g_f = None
+    if p.norm_scales is not None:
+        (g_a, g_f), g_c = _modulated_scales(combined, p), p.norm_scales[1]
     x = hidden.reshape(b * length, w)
     att, ca = block.attention, block.cross_attention
 
-    _, n = mx.add_rmsnorm_mod(x, None, _norm_weight(block.attention_norm), scale_a, shift_a, **rows, eps=eps, fmt=fmt)
+    _, n = mx.add_rmsnorm_mod(x, None, _norm_weight(block.attention_norm), scale_a, shift_a, **rows, eps=eps, fmt=fmt,
+                             global_scale=g_a)
     q, k, v = _split_heads(att, mx.matmul(n, p.qkv, out_dtype=x.dtype), b, att.num_heads, att.num_kv_heads, rope, eps)
     update = mx.matmul(mx.quantize(_attend(q, k, v, key_mask), fmt), p.out, out_dtype=x.dtype)
     gate = gate_a
     if ca is not None and context is not None and context.shape[1] > 0:
         x, n = mx.add_rmsnorm_mod(x, update, _norm_weight(block.cross_norm), gate=gate_a, **rows,
-                                  eps=block.cross_norm.eps or eps, fmt=fmt)
+                                  eps=block.cross_norm.eps or eps, fmt=fmt, global_scale=g_c)
         text = mx.quantize(context.to(x.dtype).reshape(-1, context.shape[-1]), fmt)
         q, _, _ = _split_heads(ca, mx.matmul(n, p.cross_q, out_dtype=x.dtype), b, ca.num_heads, 0, None, eps)
         _, k, v = _split_heads(ca, mx.matmul(text, p.cross_kv, out_dtype=x.dtype), b, 0, ca.num_kv_heads, None, eps)
         update = mx.matmul(mx.quantize(_attend(q, k, v, context_mask), fmt), p.cross_out, out_dtype=x.dtype)
         gate = None
     x, n = mx.add_rmsnorm_mod(x, update, _norm_weight(block.ffn_norm), scale_f, shift_f, gate=gate, **rows,
-                              eps=block.ffn_norm.eps or eps, fmt=fmt)
+                              eps=block.ffn_norm.eps or eps, fmt=fmt, global_scale=g_f)
     h = mx.matmul(n, p.up, out_dtype=x.dtype)
     if hasattr(block.feed_forward, "gate_proj"):
         gated, up = h.chunk(2, -1)

@@ -27,8 +27,12 @@ Rounding is to nearest, ties to even, saturating at the format's largest number.
   or 6), so no value saturates, kept within [-126, 126].
 * nvfp4: block scale ``amax / (6 g)`` rounded to e4m3. :func:`quantize` makes
   ``g = amax(tensor) / (6 * 448)`` from the tensor's finite values (at least
-  ``2^-100``) unless it is given one; :func:`add_rmsnorm_mod` takes ``g = 1`` unless
-  it is given one: normalised rows lie well inside e4m3's range.
+  ``2^-100``) unless it is given one; :func:`add_rmsnorm_mod` takes ``g = 1`` unless it
+  is given one. With ``g = 1`` a block whose largest value is under 0.09 gets a subnormal
+  scale (fewer bits), under 0.006 a zero one: rows that a small gain or ``1 + scale``
+  takes there want their own ``g``. No row of ``W`` columns needs a larger one than
+  ``(sqrt(W) * max|weight * (1 + scale)| + max|shift|) / 2688``, with which nothing
+  saturates and blocks keep normal scales down to 1 / 28000 of that bound.
 * A block that holds an infinity or a NaN gets a NaN scale. It reads back as NaN and
   every product row it enters is NaN; other blocks are not touched.
 """

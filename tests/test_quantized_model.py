@@ -137,6 +137,83 @@ def test_state_and_refusals() -> None:
         quantize_model(nn.ModuleList([_block(), biased]), "mxfp8")
 
 
+def _only(block: DiTBlock, branch: str) -> None:
+    """Silence the branches of ``block`` but one."""
+    last = {"attention": block.attention.out_proj, "cross": block.cross_attention.out_proj,
+            "mlp": block.feed_forward.down_proj}
+    with torch.no_grad():
+        for name, layer in last.items():
+            if name != branch:
+                layer.weight.zero_()
+
+
+# What nvfp4 may add to one branch, relative to it: an element of a block whose scale is exact
+# to e4m3's bits is off by an rms of 0.1 of the block's values; two products in a row (three in
+# the gated MLP, whose activation doubles its input's part) with two rounded operands each
+# make sqrt(6) * 0.1, and a fifth of it for what attention's weights add.
+NVFP4_BRANCH = 0.1 * 6 ** 0.5 * 1.2
+
+
+@pytest.mark.parametrize("branch", ["attention", "cross", "mlp"])
+@pytest.mark.parametrize("gain", [1.0, 0.03, 0.002])
+def test_nvfp4_norms_keep_small_gains(branch: str, gain: float) -> None:
+    """Normalised rows far below 1 keep their bits, whether the norm's weight or the modulation makes them small."""
+    torch.manual_seed(5)
+    block = _block()
+    _only(block, branch)
+    hidden, kwargs = _inputs("sample")
+    norm = {"attention": block.attention_norm, "cross": block.cross_norm, "mlp": block.ffn_norm}[branch]
+    table = block.scale_shift_table.detach().clone()
+    kwargs["modulation"][:, [0, 3]] = -table[[0, 3]]  # no shift
+    kwargs["modulation"][:, [1, 4]] = -table[[1, 4]]  # 1 + scale = 1
+    kwargs["modulation"][:, [2, 5]] = 1e4  # the branch well above the residual stream's own rounding
+    with torch.no_grad():
+        norm.weight.mul_(gain)
+        small = dict(kwargs, modulation=kwargs["modulation"].clone())
+        want = block(hidden, **kwargs) - hidden
+        quantize_model(block, "nvfp4")
+        got = block(hidden, **kwargs) - hidden
+        assert float((got - want).norm() / want.norm()) < NVFP4_BRANCH
+        if branch == "cross":
+            return
+        restore_model(block)
+        norm.weight.div_(gain)
+        small["modulation"][:, [1, 4]] += gain - 1
+        want = block(hidden, **small) - hidden
+        quantize_model(block, "nvfp4")
+        got = block(hidden, **small) - hidden
+        assert float((got - want).norm() / want.norm()) < NVFP4_BRANCH
+
+
+@pytest.mark.parametrize("form", ["sample", "grouped", "token"])
+def test_nvfp4_norms_hold_their_largest_values(form: str) -> None:
+    """A channel that carries its whole row, times a large 1 + scale, plus a large shift, does not saturate."""
+    torch.manual_seed(6)
+    block = _block()
+    _only(block, "mlp")
+    hidden, kwargs = _inputs(form)
+    hidden[..., 7] += 1000.0
+    kwargs["modulation"][..., 4, :] += 400.0
+    kwargs["modulation"][..., 3, :] += 900.0
+    with torch.no_grad():
+        want = block(hidden, **kwargs) - hidden
+        quantize_model(block, "nvfp4")
+        got = block(hidden, **kwargs) - hidden
+    assert float((got - want).norm() / want.norm()) < NVFP4_BRANCH
+
+
+def test_nvfp4_norm_scales_outlive_a_sample_that_is_not_finite() -> None:
+    torch.manual_seed(7)
+    block = _block()
+    hidden, kwargs = _inputs("sample")
+    quantize_model(block, "nvfp4")
+    with torch.no_grad():
+        for bad in (float("nan"), float("inf")):
+            kwargs["modulation"][1, 1, 3] = bad
+            out = block(hidden, **kwargs)
+            assert torch.isfinite(out[0]).all() and not torch.isfinite(out[1]).all()
+
+
 def _parallelise(block: DiTBlock, where: str) -> None:
     if where == "cp fused":
         block.attention_impl = object()
