@@ -32,7 +32,7 @@ import torch.nn.functional as F
 from torch import nn
 
 from avgen_b200.models.attention import attention
-from avgen_b200.models.rope import apply_rotary
+from avgen_b200.models.rope import RotaryTables, apply_rotary
 from avgen_b200.ops import microscale as mx
 
 _NVFP4_RANGE = 6.0 * 448.0  # largest e2m1 times largest e4m3
@@ -174,22 +174,29 @@ def _heads(rows: torch.Tensor, batch: int, heads: int, norm: nn.Module) -> torch
 def _split_heads(module: nn.Module, rows: torch.Tensor, batch: int, heads: int, kv_heads: int, rope,  # noqa: ANN001
                  eps: float) -> tuple[torch.Tensor | None, torch.Tensor | None, torch.Tensor | None]:
     """Query, key and value heads ``[B, H, L, D]`` of packed projection rows (either may have none)."""
+    coords = freq = axis = tables = None
+    if isinstance(rope, RotaryTables):
+        tables = rope
+    elif rope is not None:
+        if rows.is_cuda:  # the kernel forms the angles itself
+            coords, freq, axis = rope.kernel_args()
+        else:
+            tables = rope.tables()
+    d = module.head_dim
     if rows.is_cuda:
         from avgen_b200.ops import kernels as K
 
-        coords, freq, axis = rope.kernel_args() if rope is not None else (None, None, None)
         normed = isinstance(module.q_norm, nn.RMSNorm)
-        return K.qkv_rope(rows, batch=batch, length=rows.shape[0] // batch, heads=heads, kv_heads=kv_heads,
-                          head_dim=module.head_dim, q_weight=_norm_weight(module.q_norm) if normed and heads else None,
-                          k_weight=_norm_weight(module.k_norm) if normed and kv_heads else None, coords=coords,
-                          freq=freq, axis=axis, eps=eps)
-    d = module.head_dim
-    q, k, v = rows.split((heads * d, kv_heads * d, kv_heads * d), -1)
-    q = _heads(q, batch, heads, module.q_norm) if heads else None
-    k = _heads(k, batch, kv_heads, module.k_norm) if kv_heads else None
-    v = _heads(v, batch, kv_heads, nn.Identity()) if kv_heads else None
-    if rope is not None:
-        tables = rope.tables()
+        q, k, v = K.qkv_rope(rows, batch=batch, length=rows.shape[0] // batch, heads=heads, kv_heads=kv_heads,
+                             head_dim=d, q_weight=_norm_weight(module.q_norm) if normed and heads else None,
+                             k_weight=_norm_weight(module.k_norm) if normed and kv_heads else None, coords=coords,
+                             freq=freq, axis=axis, eps=eps)
+    else:
+        q, k, v = rows.split((heads * d, kv_heads * d, kv_heads * d), -1)
+        q = _heads(q, batch, heads, module.q_norm) if heads else None
+        k = _heads(k, batch, kv_heads, module.k_norm) if kv_heads else None
+        v = _heads(v, batch, kv_heads, nn.Identity()) if kv_heads else None
+    if tables is not None:
         q, k = apply_rotary(q, tables), apply_rotary(k, tables)
     return q, k, v
 

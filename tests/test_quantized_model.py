@@ -214,6 +214,27 @@ def test_nvfp4_norm_scales_outlive_a_sample_that_is_not_finite() -> None:
             assert torch.isfinite(out[0]).all() and not torch.isfinite(out[1]).all()
 
 
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_rotary_tables_do_what_their_coordinates_do(device: str) -> None:
+    torch.manual_seed(8)
+    block = _block()
+    _only(block, "attention")
+    dtype = torch.float32 if device == "cpu" else torch.bfloat16
+    hidden, kwargs = _inputs("sample", device, dtype)
+    kwargs["rope"].coords.mul_(4.0)
+    kwargs["modulation"][:, 2] = 1e2
+    block.to(device)
+    quantize_model(block, "mxfp8")
+    with torch.no_grad():
+        want = (block(hidden, **kwargs) - hidden).float()
+        got = (block(hidden, **dict(kwargs, rope=kwargs["rope"].tables())) - hidden).float()
+        none = (block(hidden, **dict(kwargs, rope=None)) - hidden).float()
+    off = float((got - want).norm() / want.norm())
+    # the same numbers on the CPU; on a GPU the heads are rounded to bf16 once more before they are rotated
+    assert off == 0 if device == "cpu" else off < 2 ** -5
+    assert float((none - want).norm() / want.norm()) > 2 ** -2
+
+
 def _parallelise(block: DiTBlock, where: str) -> None:
     if where == "cp fused":
         block.attention_impl = object()
