@@ -84,10 +84,6 @@ def _check(block: nn.Module, name: str) -> None:
     biased = [n for n, m in linears.items() if m.bias is not None]
     if biased:
         raise ValueError(f"{name}: quantised linears have no bias; found {', '.join(biased)}")
-    cuda = next(block.parameters()).is_cuda
-    heads = [block.attention.head_dim] + ([block.cross_attention.head_dim] if block.cross_attention is not None else [])
-    if cuda and any(d != 128 for d in heads):
-        raise ValueError(f"{name}: the attention kernels take head dim 128; got {heads}")
 
 
 def _weight(layer: nn.Linear) -> torch.Tensor:
@@ -166,6 +162,12 @@ def _norm_weight(norm: nn.Module) -> torch.Tensor | None:
     return None if w is None else w.detach().float().contiguous()
 
 
+def _on_kernels(t: torch.Tensor, head_dim: int) -> bool:
+    """Whether heads run on the fused block's kernels; any other head dim takes what the plain
+    block's layers take, which on a GPU is :func:`attention`'s refusal."""
+    return t.is_cuda and head_dim == 128
+
+
 def _heads(rows: torch.Tensor, batch: int, heads: int, norm: nn.Module) -> torch.Tensor:
     """``[B*L, H*D]`` rows -> ``[B, H, L, D]``, normalised per head."""
     return norm(rows.view(batch, -1, heads, rows.shape[-1] // heads).transpose(1, 2))
@@ -175,15 +177,16 @@ def _split_heads(module: nn.Module, rows: torch.Tensor, batch: int, heads: int, 
                  eps: float) -> tuple[torch.Tensor | None, torch.Tensor | None, torch.Tensor | None]:
     """Query, key and value heads ``[B, H, L, D]`` of packed projection rows (either may have none)."""
     coords = freq = axis = tables = None
+    kernels = _on_kernels(rows, module.head_dim)
     if isinstance(rope, RotaryTables):
         tables = rope
     elif rope is not None:
-        if rows.is_cuda:  # the kernel forms the angles itself
+        if kernels:  # the kernel forms the angles itself
             coords, freq, axis = rope.kernel_args()
         else:
             tables = rope.tables()
     d = module.head_dim
-    if rows.is_cuda:
+    if kernels:
         from avgen_b200.ops import kernels as K
 
         normed = isinstance(module.q_norm, nn.RMSNorm)
@@ -203,7 +206,7 @@ def _split_heads(module: nn.Module, rows: torch.Tensor, batch: int, heads: int, 
 
 def _attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: torch.Tensor | None) -> torch.Tensor:
     """Token-major attention output as rows ``[B*L, H*D]``."""
-    if q.is_cuda:
+    if _on_kernels(q, q.shape[-1]):
         from avgen_b200.ops import kernels as K
 
         out, _ = K.attention_fwd(q, k, v, kmask=K.pack_key_mask(mask), scale=1.0 / math.sqrt(q.shape[-1]),

@@ -334,3 +334,39 @@ def test_gpu_model_samples_quantised() -> None:
     packed = pipe(["a kite"], seed=1).video.float()
     assert torch.isfinite(packed).all()
     assert float((packed - full).norm() / full.norm()) < 0.2
+
+
+@pytest.mark.gpu
+def test_gpu_model_quantises_beside_blocks_of_other_head_dims() -> None:
+    """A joint model whose audio tower has heads the kernels do not take: video alone samples, as unquantised."""
+    from dataclasses import asdict
+
+    from avgen_b200.codecs import ReferenceTextEncoder, ReferenceVideoCodec
+    from avgen_b200.infer import GenerationConfig, GenerationPipeline, ScheduleConfig
+    from avgen_b200.models import build_model, preset
+
+    torch.manual_seed(9)
+    cfg = {k: v for k, v in asdict(preset("tiny_gpu")).items() if k != "rope_scaling"}
+    cfg.update(audio_width=128, audio_num_heads=2, audio_in_channels=4, audio_ffn_hidden=256)
+    model = build_model("av_dit", cfg).cuda().eval()
+    model.init_weights()
+    video = ReferenceVideoCodec(channels=cfg["in_channels"], temporal_compression=1, spatial_compression=1)
+    text = ReferenceTextEncoder(width=cfg["text_width"], max_length=16)
+    settings = GenerationConfig(steps=2, height=32, width=32, num_frames=4, schedule=ScheduleConfig(steps=2),
+                                generate_audio=False)
+    pipe = GenerationPipeline(model, video_codec=video, text_encoder=text, config=settings, device=torch.device("cuda"))
+    assert torch.isfinite(pipe(["a kite"], seed=1).video).all()
+    assert quantize_model(model, "mxfp8") == 2 * cfg["depth"]
+    assert torch.isfinite(pipe(["a kite"], seed=1).video).all()
+
+
+@pytest.mark.gpu
+def test_gpu_block_of_another_head_dim_refuses_when_it_runs() -> None:
+    block = DiTBlock(256, 4, hidden=512).cuda()
+    hidden, kwargs = _inputs("sample", "cuda", torch.bfloat16)
+    kwargs["rope"] = None
+    for pack in (False, True):
+        if pack:
+            quantize_model(block, "mxfp8")
+        with torch.no_grad(), pytest.raises(NotImplementedError, match="head_dim 128"):
+            block(hidden, **kwargs)
