@@ -245,6 +245,8 @@ def quantized_block_forward(block: nn.Module, hidden: torch.Tensor, combined: to
     if p.norm_scales is not None:
         (g_a, g_f), g_c = _modulated_scales(combined, p), p.norm_scales[1]
     x = hidden.reshape(b * length, w)
+    if x.is_cuda:
+        x = x.to(torch.bfloat16)  # the fused block's residual stream, whatever type comes in
     att, ca = block.attention, block.cross_attention
 
     _, n = mx.add_rmsnorm_mod(x, None, _norm_weight(block.attention_norm), scale_a, shift_a, **rows, eps=eps, fmt=fmt,
@@ -273,4 +275,4 @@ def quantized_block_forward(block: nn.Module, hidden: torch.Tensor, combined: to
         out = torch.addcmul(x.float(), gate_f[groups.long()], update)
     else:
         out = torch.addcmul(x.float().view(-1, per, w), gate_f[:, None], update.view(-1, per, w))
-    return out.to(hidden.dtype).view(b, length, w)
+    return out.to(x.dtype).to(hidden.dtype).view(b, length, w)

@@ -370,3 +370,19 @@ def test_gpu_block_of_another_head_dim_refuses_when_it_runs() -> None:
             quantize_model(block, "mxfp8")
         with torch.no_grad(), pytest.raises(NotImplementedError, match="head_dim 128"):
             block(hidden, **kwargs)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_gpu_block_takes_other_types_as_the_plain_block_does(dtype: torch.dtype) -> None:
+    torch.manual_seed(10)
+    block = _block().cuda()
+    hidden, kwargs = _inputs("sample", "cuda", torch.bfloat16)
+    hidden, kwargs["context"] = hidden.to(dtype), kwargs["context"].to(dtype)
+    with torch.no_grad():
+        for pack in (False, True):
+            if pack:
+                quantize_model(block, "nvfp4")
+            out = block(hidden, **kwargs)
+            assert out.dtype is dtype
+            assert torch.equal(out, block(hidden.bfloat16(), **kwargs).to(dtype))
