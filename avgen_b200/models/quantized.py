@@ -235,9 +235,11 @@ def quantized_block_forward(block: nn.Module, hidden: torch.Tensor, combined: to
     fmt, eps = p.fmt, block.attention_norm.eps or 1e-6
     groups, per = None, length
     if mod_index is not None:
-        groups = mod_index.reshape(-1).to(torch.int32).contiguous()
+        groups = mod_index.expand(b, length).reshape(-1).to(torch.int32).contiguous()
     elif combined.ndim == 4:
-        combined, per = combined.reshape(b * length, *combined.shape[2:]), 1
+        combined, per = combined.expand(b, length, *combined.shape[2:]).reshape(b * length, *combined.shape[2:]), 1
+    else:
+        combined = combined.expand(b, *combined.shape[1:])
     rows = {"rows_per_batch": per, "groups": groups}
     combined = combined.float().contiguous()
     shift_a, scale_a, gate_a, shift_f, scale_f, gate_f = combined.unbind(1)

@@ -235,6 +235,27 @@ def test_rotary_tables_do_what_their_coordinates_do(device: str) -> None:
     assert float((none - want).norm() / want.norm()) > 2 ** -2
 
 
+@pytest.mark.parametrize("form", ["sample", "grouped", "token", "frame"])
+def test_modulation_shared_by_the_batch(form: str) -> None:
+    """Modulation (or its row numbers) of one sample stands for all, as in the plain block."""
+    torch.manual_seed(11)
+    block = _block()
+    hidden, kwargs = _inputs("token" if form == "frame" else form)
+    full = dict(kwargs)
+    if form == "grouped":
+        kwargs["modulation_index"] = kwargs["modulation_index"][:1]
+        full["modulation_index"] = kwargs["modulation_index"].expand(2, 160).contiguous()
+    else:
+        one = kwargs["modulation"][:, :1] if form == "frame" else kwargs["modulation"][:1]
+        full["modulation"] = one.expand_as(kwargs["modulation"]).contiguous()
+        kwargs["modulation"] = one
+    with torch.no_grad():
+        assert torch.equal(block(hidden, **kwargs), block(hidden, **full))
+        for fmt in ("mxfp8", "nvfp4"):
+            quantize_model(block, fmt)
+            assert torch.equal(block(hidden, **kwargs), block(hidden, **full))
+
+
 def _parallelise(block: DiTBlock, where: str) -> None:
     if where == "cp fused":
         block.attention_impl = object()
