@@ -256,6 +256,177 @@ def test_modulation_shared_by_the_batch(form: str) -> None:
             assert torch.equal(block(hidden, **kwargs), block(hidden, **full))
 
 
+# ----------------------------------------------------------------------------- every part of a block
+def _marked_block(ffn: str) -> DiTBlock:
+    """A block whose every part has a large share in its output."""
+    block = _block(ffn=ffn)
+    with torch.no_grad():
+        for m in block.modules():
+            if isinstance(m, nn.Linear):
+                m.weight.normal_(std=m.in_features ** -0.5)
+        for norm in (block.attention_norm, block.cross_norm, block.ffn_norm):
+            norm.weight.uniform_(0.5, 1.5)
+        for att in (block.attention, block.cross_attention):
+            att.q_norm.weight.uniform_(2.0, 3.0)  # attention that looks at a few keys
+            att.k_norm.weight.uniform_(0.5, 1.5)
+            att.out_proj.weight.mul_(2.0)
+        block.scale_shift_table.normal_(std=0.5)
+    return block
+
+
+class _Reference:
+    """The parts of a block in 64 bits, each from the packed operands and stored rows the block itself had."""
+
+    def __init__(self, block: DiTBlock, kwargs: dict) -> None:
+        self.block, self.kwargs = block, kwargs
+        mod = (kwargs["modulation"] + block.scale_shift_table.detach()).double()
+        if kwargs["modulation_index"] is not None:
+            mod = mod[kwargs["modulation_index"].long()]
+        elif mod.ndim == 3:
+            mod = mod[:, None].expand(-1, 160, -1, -1)
+        self.mod = mod.reshape(320, 6, 256).unbind(1)
+
+    def norm(self, x: torch.Tensor, norm: nn.Module, chunk: int | None) -> torch.Tensor:
+        y = x / torch.sqrt(x.square().mean(-1, keepdim=True) + 1e-6) * norm.weight.detach().double()
+        return y if chunk is None else y * (1 + self.mod[chunk + 1]) + self.mod[chunk]
+
+    def attention(self, att: nn.Module, q: torch.Tensor, kv: torch.Tensor, *, rope: bool,
+                  mask: torch.Tensor | None) -> torch.Tensor:
+        def heads(rows: torch.Tensor, norm: nn.Module | None) -> torch.Tensor:
+            t = rows.view(2, -1, 2, 128).transpose(1, 2)
+            if norm is None:
+                return t
+            return t / torch.sqrt(t.square().mean(-1, keepdim=True) + 1e-6) * norm.weight.detach().double()
+
+        def turn(t: torch.Tensor) -> torch.Tensor:
+            tables = self.kwargs["rope"].tables()
+            z = torch.view_as_complex(t.reshape(*t.shape[:-1], 64, 2))
+            return torch.view_as_real(z * torch.complex(tables.cos.double(), tables.sin.double())).flatten(-2)
+
+        q, k, v = heads(q, att.q_norm), heads(kv[:, :256], att.k_norm), heads(kv[:, 256:], None)
+        if rope:
+            q, k = turn(q), turn(k)
+        s = q @ k.transpose(-1, -2) / 128 ** 0.5
+        if mask is not None:
+            s = s.masked_fill(~mask[:, None, None], float("-inf"))
+        return (torch.softmax(s, -1) @ v).transpose(1, 2).reshape(320, 256)
+
+    def activation(self, h: torch.Tensor) -> torch.Tensor:
+        if hasattr(self.block.feed_forward, "gate_proj"):
+            gate, up = h.chunk(2, -1)
+            return nn.functional.silu(gate) * up
+        return nn.functional.gelu(h, approximate="tanh")
+
+
+def _tape(monkeypatch: pytest.MonkeyPatch) -> list:
+    """The operators' calls of a quantised block, in order: (arguments, result)."""
+    import types
+
+    from avgen_b200.models import quantized
+
+    calls: list = []
+
+    def kept(name: str):  # noqa: ANN202
+        def call(*args: object, **more: object) -> object:
+            out = getattr(mx, name)(*args, **more)
+            calls.append((args, out))
+            return out
+
+        return call
+
+    names = ("quantize", "matmul", "add_rmsnorm_mod")
+    monkeypatch.setattr(quantized, "mx", types.SimpleNamespace(**{name: kept(name) for name in names}))
+    return calls
+
+
+def _off(got: torch.Tensor, want: torch.Tensor) -> float:
+    got = got.detach().double().cpu().reshape(want.shape)
+    return float((got - want).norm() / want.norm())
+
+
+# What a stage may be off, relative to its norm, from the 64-bit one on the same operands. On the
+# CPU: sums of up to 512 fp32 products and their functions. On a GPU: up to five roundings to
+# bf16 of 2^-9 / sqrt(3) each, of which those of q and k reach attention's scores times their
+# size (2.5) and come out averaged; rows that are stored are rounded once or twice.
+STAGE = {"cpu": 1e-5, "cuda": 2.0 ** -6}
+STORED = {"cpu": 1e-5, "cuda": 2.0 ** -8}
+# Packed values beside the packed 64-bit ones: an element that crosses a rounding boundary is a
+# spacing off; fp32 arithmetic moves at most one in 10^4 there.
+PACKED = 1e-2
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("fmt", mx.FORMATS)
+@pytest.mark.parametrize("ffn,form", [("swiglu", "sample"), ("gelu", "grouped"), ("swiglu", "token")])
+def test_every_part_of_a_block(fmt: str, ffn: str, form: str, device: str, monkeypatch: pytest.MonkeyPatch) -> None:
+    """Each stage of the block against 64 bits, within far less than any part of it (rotation, masks, each
+    modulation, residuals) adds."""
+    torch.manual_seed(12)
+    block = _marked_block(ffn)
+    hidden, kwargs = _inputs(form)
+    kwargs["modulation"] = 0.5 * torch.randn_like(kwargs["modulation"])
+    kwargs["modulation"][..., [2, 5], :] += 1.0
+    hidden, kwargs["context"] = hidden.bfloat16().float(), kwargs["context"].bfloat16().float()
+    ref = _Reference(copy.deepcopy(block), kwargs)
+    dtype = torch.float32 if device == "cpu" else torch.bfloat16
+    block.to(device)
+    quantize_model(block, fmt)
+    calls = _tape(monkeypatch)
+    given = {k: v.to(device) if isinstance(v, torch.Tensor) else v for k, v in kwargs.items()}
+    given["rope"] = RopeInputs(kwargs["rope"].coords.to(device), kwargs["rope"].rope)
+    given["context"] = given["context"].to(dtype)
+    with torch.no_grad():
+        out = block(hidden.to(device, dtype), **given)
+
+    norm1, qkv, pack1, out1, norm2, text, cq, ckv, pack2, out2, norm3, up, pack3, down = calls
+    p, ca = block.quantized, ref.block.cross_attention
+    weight = {n: oracle.decode(getattr(p, n)) for n in ("qkv", "out", "cross_q", "cross_kv", "cross_out", "up", "down")}
+    x = [hidden.double().view(320, 256)] + [call[1][0].double().cpu() for call in (norm2, norm3)]
+    tight, stored = STAGE[device], STORED[device]
+
+    # the packed norms
+    for i, (call, norm, chunk) in enumerate(((norm1, ref.block.attention_norm, 0), (norm2, ref.block.cross_norm, None),
+                                             (norm3, ref.block.ffn_norm, 3))):
+        y, t = ref.norm(x[i], norm, chunk), call[1][1]
+        if i > 0 and device == "cuda":  # they take the fp32 sum, of which x holds the rounding to bf16
+            y = ref.norm(call[0][0].double().cpu() + call[0][1].double().cpu() * (ref.mod[2] if i == 1 else 1.0), norm,
+                         chunk)
+        g = None if t.global_scale is None else t.global_scale.cpu()
+        assert _off(oracle.decode(t), oracle.decode(mx.quantize(y.float(), fmt, global_scale=g))) < PACKED
+        if chunk is not None:
+            for part in (0, 1):
+                assert _off(y - ref.mod[chunk] if part == 0 else ref.norm(x[i], norm, None), y) > 0.1
+    # self-attention
+    rows = oracle.decode(norm1[1][1]) @ weight["qkv"].t()
+    want = ref.attention(ref.block.attention, rows[:, :256], rows[:, 256:], rope=True, mask=kwargs["key_mask"])
+    assert _off(pack1[0][0], want) < tight
+    for rope, mask in ((False, kwargs["key_mask"]), (True, None)):
+        assert _off(ref.attention(ref.block.attention, rows[:, :256], rows[:, 256:], rope=rope, mask=mask), want) > 0.1
+    # its projection and gated residual
+    update = oracle.decode(pack1[1]) @ weight["out"].t()
+    assert _off(out1[1], update) < stored and _off(x[1], x[0] + ref.mod[2] * update) < stored
+    assert _off(x[0] + update, x[1]) > 0.1
+    # cross-attention, its projection and residual
+    assert _off(oracle.decode(text[1]), oracle.decode(mx.quantize(kwargs["context"].view(-1, 256), fmt))) == 0
+    q = oracle.decode(norm2[1][1]) @ weight["cross_q"].t()
+    kv = oracle.decode(text[1]) @ weight["cross_kv"].t()
+    want = ref.attention(ca, q, kv, rope=False, mask=kwargs["context_mask"])
+    assert _off(pack2[0][0], want) < tight
+    assert _off(ref.attention(ca, q, kv, rope=False, mask=None), want) > 0.05
+    update = oracle.decode(pack2[1]) @ weight["cross_out"].t()
+    assert _off(out2[1], update) < stored and _off(x[2], x[1] + update) < stored
+    # the MLP and its gated residual
+    assert _off(pack3[0][0], ref.activation(oracle.decode(norm3[1][1]) @ weight["up"].t())) < tight
+    update = oracle.decode(pack3[1]) @ weight["down"].t()
+    assert _off(down[1], update) < stored and _off(out, x[2] + ref.mod[5] * update) < stored
+    assert _off(x[2] + update, out.double().cpu().view(320, 256)) > 0.1
+    # nothing between the stages: each reads what the one before wrote
+    for a, b in ((norm1[1][1], qkv[0][0]), (pack1[1], out1[0][0]), (out1[1], norm2[0][1]), (norm2[1][1], cq[0][0]),
+                 (text[1], ckv[0][0]), (pack2[1], out2[0][0]), (out2[1], norm3[0][1]), (norm2[1][0], norm3[0][0]),
+                 (norm3[1][1], up[0][0]), (pack3[1], down[0][0])):
+        assert a is b
+
+
 def _parallelise(block: DiTBlock, where: str) -> None:
     if where == "cp fused":
         block.attention_impl = object()
