@@ -161,6 +161,39 @@ def test_add_rmsnorm_types_and_missing_parts(dtype: torch.dtype, cols: int) -> N
         _check_norm({k: None if k in missing else v for k, v in case.items()}, "mxfp8", eps=1e-5)
 
 
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("cols", [250, 256, 500, 700, 1000, 4096, 9000, 20000])
+def test_add_rmsnorm_other_types_to_four_bits(fmt: str, dtype: torch.dtype, cols: int) -> None:
+    case = _norm_case(130 if cols < 5000 else 5, cols, dtype, 2, seed=cols)
+    _check_norm(case, fmt)
+    _check_norm({k: None if k in ("scale", "shift", "gate", "groups") else v for k, v in case.items()}, fmt)
+
+
+@pytest.mark.parametrize("cols", [640, 1001])
+@pytest.mark.parametrize("gain", [1.0, 1e-2, 1e-3])
+def test_add_rmsnorm_nvfp4_tensor_scale_of_the_norms_range(cols: int, gain: float) -> None:
+    """With the tensor scale that the largest possible value of a row asks for, block scales keep e4m3's
+    precision (normal ones 2^-4 of theirs), and values an element's, at gains that differ by 1000."""
+    case = _norm_case(70, cols, torch.bfloat16, 3, seed=cols)
+    case["shift"] = None
+    case["weight"][:cols // 2] *= gain
+    reach = cols ** 0.5 * float((case["weight"].abs() * (1 + case["scale"]).abs()).max())
+    g = torch.tensor([reach / 2688])
+    dev = {k: None if v is None else v.to(DEV) for k, v in case.items()}
+    _, t = mx.add_rmsnorm_mod(dev["x"], dev["update"], dev["weight"], dev["scale"], gate=dev["gate"],
+                              groups=dev["groups"], fmt="nvfp4", global_scale=g.to(DEV))
+    assert torch.equal(t.global_scale.cpu(), g)
+    y = _norm_oracle(case, 1e-6)[1]
+    amax = torch.nn.functional.pad(y.abs(), (0, -cols % 16)).view(len(y), -1, 16).amax(-1) / (6 * g.double())
+    assert ((oracle.e4m3(oracle.scale_bytes(t)) - amax).abs() <= amax * (2.0 ** -4 + 1e-5) + 2.0 ** -10).all()
+    scale = oracle.scales(t)
+    ratio = torch.where(scale > 0, y / scale, torch.zeros(()).double())
+    slack = 1e-5 * amax.repeat_interleave(16, 1)[:, :cols] * 6 * g.double()
+    assert ((oracle.elements(t) - ratio.clamp(-6, 6)).abs() * scale
+            <= 0.5 * oracle.spacing(ratio, "nvfp4") * scale + slack).all()
+
+
 def test_add_rmsnorm_rows_per_batch_and_strides() -> None:
     case = _norm_case(64, 640, torch.bfloat16, 4, seed=3)
     case["groups"] = None
