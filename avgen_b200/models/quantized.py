@@ -52,9 +52,10 @@ class QuantizedBlock:
     cross_q: mx.MXTensor | None = None
     cross_kv: mx.MXTensor | None = None
     cross_out: mx.MXTensor | None = None
-    # nvfp4: tensor scales [1] that hold the whole range of an un-modulated norm's output
-    # (self-attention's, cross-attention's and the MLP's); None for the other formats
-    norm_scales: tuple[torch.Tensor, torch.Tensor | None, torch.Tensor] | None = None
+    # nvfp4: tensor scales that hold the whole range of the norms' output, [2] before modulation
+    # (self-attention's and the MLP's) and [1] of cross-attention's; None for the other formats
+    norm_scales: torch.Tensor | None = None
+    cross_scale: torch.Tensor | None = None
 
     @property
     def nbytes(self) -> int:
@@ -106,10 +107,9 @@ def _modulated_scales(combined: torch.Tensor, p: QuantizedBlock) -> tuple[torch.
     1 / 28000 of that bound keep normal scales. A modulation that is not finite (its rows are
     NaN in any case) counts as 2, so that other rows stay what they are."""
     if len(combined) == 0:
-        return p.norm_scales[0], p.norm_scales[2]
+        return p.norm_scales[:1], p.norm_scales[1:]
     peak = torch.linalg.vector_norm(combined, float("inf"), dim=(0, 2)).nan_to_num(nan=2.0, posinf=2.0)  # [6]
-    own = torch.cat((p.norm_scales[0], p.norm_scales[2]))
-    g = torch.addcmul(own, own, peak[1::3]).add_(peak[0::3], alpha=1.0 / _NVFP4_RANGE)
+    g = torch.addcmul(p.norm_scales, p.norm_scales, peak[1::3]).add_(peak[0::3], alpha=1.0 / _NVFP4_RANGE)
     return g[:1], g[1:]
 
 
@@ -138,9 +138,10 @@ def quantize_model(model: nn.Module, fmt: str = "mxfp8") -> int:
                         "cross_out": _pack(fmt, ca.out_proj)}
             if fmt == "nvfp4":
                 device = att.q_proj.weight.device
-                more["norm_scales"] = (_norm_scale(block.attention_norm, block.width, device),
-                                       _norm_scale(block.cross_norm, block.width, device) if ca is not None else None,
-                                       _norm_scale(block.ffn_norm, block.width, device))
+                more["norm_scales"] = torch.cat([_norm_scale(n, block.width, device)
+                                                 for n in (block.attention_norm, block.ffn_norm)])
+                if ca is not None:
+                    more["cross_scale"] = _norm_scale(block.cross_norm, block.width, device)
             block.quantized = QuantizedBlock(fmt, qkv=_pack(fmt, att.q_proj, att.k_proj, att.v_proj),
                                              out=_pack(fmt, att.out_proj), up=_pack(fmt, *up),
                                              down=_pack(fmt, ff.down_proj), **more)
@@ -243,9 +244,9 @@ def quantized_block_forward(block: nn.Module, hidden: torch.Tensor, combined: to
     rows = {"rows_per_batch": per, "groups": groups}
     combined = combined.float().contiguous()
     shift_a, scale_a, gate_a, shift_f, scale_f, gate_f = combined.unbind(1)
-    g_a = g_c = g_f = None
+    g_a = g_f = None
     if p.norm_scales is not None:
-        (g_a, g_f), g_c = _modulated_scales(combined, p), p.norm_scales[1]
+        g_a, g_f = _modulated_scales(combined, p)
     x = hidden.reshape(b * length, w)
     if x.is_cuda:
         x = x.to(torch.bfloat16)  # the fused block's residual stream, whatever type comes in
@@ -258,7 +259,7 @@ def quantized_block_forward(block: nn.Module, hidden: torch.Tensor, combined: to
     gate = gate_a
     if ca is not None and context is not None and context.shape[1] > 0:
         x, n = mx.add_rmsnorm_mod(x, update, _norm_weight(block.cross_norm), gate=gate_a, **rows,
-                                  eps=block.cross_norm.eps or eps, fmt=fmt, global_scale=g_c)
+                                  eps=block.cross_norm.eps or eps, fmt=fmt, global_scale=p.cross_scale)
         text = mx.quantize(context.to(x.dtype).reshape(-1, context.shape[-1]), fmt)
         q, _, _ = _split_heads(ca, mx.matmul(n, p.cross_q, out_dtype=x.dtype), b, ca.num_heads, 0, None, eps)
         _, k, v = _split_heads(ca, mx.matmul(text, p.cross_kv, out_dtype=x.dtype), b, 0, ca.num_kv_heads, None, eps)

@@ -470,6 +470,60 @@ def test_context_parallelism_over_packed_blocks_is_refused() -> None:
         model[0](hidden, **kwargs)
 
 
+def _two_ranks(rank: int, port: int) -> None:
+    import os
+
+    import torch.distributed as dist
+    from torch.distributed.device_mesh import init_device_mesh
+    from torch.distributed.fsdp import fully_shard
+
+    from avgen_b200.parallel.context import apply_context_parallel
+    from avgen_b200.parallel.tensor import apply_tensor_parallel
+
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+    dist.init_process_group("gloo", rank=rank, world_size=2)
+    mesh = init_device_mesh("cpu", (2,), mesh_dim_names=("tp",))
+
+    def packed() -> tuple[nn.Module, torch.Tensor, dict]:
+        torch.manual_seed(13)
+        model = nn.Module()
+        model.blocks = nn.ModuleList([_block()])
+        hidden, kwargs = _inputs("sample")
+        quantize_model(model, "mxfp8")
+        return model, hidden, kwargs
+
+    with torch.no_grad():
+        model, hidden, kwargs = packed()
+        want = model.blocks[0](hidden, **kwargs)
+        for apply in (lambda m: apply_tensor_parallel(m, mesh, style="dtensor"),
+                      lambda m: fully_shard(m.blocks[0], mesh=mesh)):
+            model = packed()[0]
+            apply(model)
+            with pytest.raises(ValueError, match="sharded weights"):
+                quantize_model(model, "mxfp8")
+            assert torch.equal(model.blocks[0](hidden, **kwargs), want)
+        for apply, kind in ((lambda m: apply_tensor_parallel(m, mesh, style="heads"), "tensor"),
+                            (lambda m: apply_tensor_parallel(m, mesh, style="heads", sequence_parallel=True), "tensor"),
+                            (lambda m: apply_context_parallel(m, mesh), "context")):
+            model = packed()[0]
+            apply(model)
+            with pytest.raises(RuntimeError, match=f"{kind} parallelism"):
+                model.blocks[0](hidden, **kwargs)
+    dist.destroy_process_group()
+
+
+def test_packed_blocks_on_two_ranks() -> None:
+    """What leaves a block's call whole (DTensor plans, FSDP2) gives its result; what splits it is refused."""
+    import socket
+
+    import torch.multiprocessing as mp
+
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    mp.spawn(_two_ranks, args=(port,), nprocs=2, join=True)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("fmt", mx.FORMATS)
 @pytest.mark.parametrize("ffn,form", [("swiglu", "sample"), ("gelu", "grouped"), ("swiglu", "token")])
