@@ -442,7 +442,7 @@ struct MxNormDesc {
   uint8_t* scales = nullptr;
   const float* g = nullptr;
 };
-constexpr int kMxNormMaxCols = 65536;  // a row stays in one CTA's registers
+constexpr int kMxNormMaxCols = 65536;  // a row stays on one SM (above 16384 columns partly in spilled registers)
 long mx_norm_max_rows(int device);     // above it the kernel's row numbers would overflow
 void mx_add_rmsnorm_launch(const MxNormDesc& d, cudaStream_t stream);
 

@@ -14,8 +14,10 @@
 //              with its own 134; fp32 13824 x 5120 to mxfp4 54 (6.0); 20000 x 5001 to
 //              mxfp4, rows not aligned, 69 (3.7)
 //   read back  mxfp8 85 (6.0), 4 bits 74 (5.8); 20000 x 5001 from mxfp4 60 (4.2)
-//   norm       to mxfp8 192 (6.1), with two modulation levels 221 (5.3); 16387 x 5120 99
-//              (5.9); 20000 x 5001, whose rows are not aligned, 227 (3.1)
+//   norm       to mxfp8 192 to 203 (6.1 to 5.8), with two modulation levels 203 to 221; to
+//              mxfp4 173 (6.3) and 200, to nvfp4 186 (5.9) and 223; of fp32 rows to mxfp8 354
+//              (6.2) and 365; 16387 x 5120 95 (6.2) and 111; 20000 x 5001, whose rows are not
+//              aligned, 227 (3.1) and 309; 4096 x 40000 476 (2.4) and 793, of fp32 930 and 1089
 #include <algorithm>
 #include <limits>
 
@@ -593,11 +595,16 @@ __device__ __forceinline__ float inverse_root(float x) {
   return fabsf(e) < 0.5f ? fmaf(0.5f * r, e, r) : r;
 }
 
-// A row is held in registers, CHUNKS x 8 columns per lane, between its sum of squares
-// and its store: x and the update are read once. Rows of up to 1024 columns take one
+// A row is held on its SM, CHUNKS x 8 columns per lane, between its sum of squares
+// and its store: x and the update are read once. Rows of up to 768 columns take one
 // warp each (WARP_ROWS) and no barrier; longer ones a CTA, with one barrier per row. The
 // next row's x and update are requested before the reduction, so that loads stay in
 // flight through it.
+//
+// Up to 16384 columns that is in registers, but for fp32 rows and modulated 16-bit ones of no
+// alignment, which spill up to 450 bytes a thread (16-bit ones of 257 to 512 columns 64). Wider
+// rows (8 chunks) take 1024 threads of 64 registers, as many as their own 64 values: they
+// spill 0.7 to 1.5 KB a thread, of fp32 1.8 to 3.2 KB, and run at 1.4 to 2.4 TB/s.
 //
 // The norm takes the fp32 sum x + gate * update, not its rounding to T; statistics,
 // modulation and scaling stay in fp32 until the codes.

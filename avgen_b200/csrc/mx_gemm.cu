@@ -23,13 +23,14 @@
 // operand bytes from L2 and shared memory per product as one SM would need for half
 // the work.
 //
-// What bounds it: an SM takes in about 52 bytes a clock through TMA here, so a k-block of
-// 34 to 38 KB takes some 650 clocks, against 512 for its products; with both at once it
-// measured 750 to 780 whatever the ring's depth beyond four stages. Short K adds the
-// store of the output (19 % at K = 2560). Measured on a B200 at its 1 kW power limit:
-//   65536 x 20480 x 2560 nvfp4   1.75 ms, 3.9 PFLOP/s (4.7 before the limit sets in)
-//   16384 x 2560 x 10240 mxfp4   165 us, 5.2 PFLOP/s (6.1)
-//   32768 x 5120 x 5120 mxfp8    686 us, 2.5 PFLOP/s (2.9)
+// What bounds it, as far as it was taken apart (mxfp8, 40 k-blocks): an SM takes in about 52
+// bytes a clock through TMA here, so a k-block of 34 to 38 KB takes some 650 clocks, against
+// 512 for its products; with both at once it measured 750 to 780 whatever the ring's depth
+// beyond four stages. Short K adds the store of the output (19 % at K = 2560 in nvfp4, ten
+// k-blocks, where the roles' waits were not measured). Times on a B200 at its 1 kW power limit:
+//   65536 x 20480 x 2560 nvfp4   1.75 to 1.84 ms, 3.9 to 3.7 PFLOP/s (4.7 before the limit sets in)
+//   16384 x 2560 x 10240 mxfp4   165 to 172 us, 5.2 to 5.0 PFLOP/s (6.1)
+//   32768 x 5120 x 5120 mxfp8    686 to 731 us, 2.5 to 2.4 PFLOP/s (2.9)
 #include <algorithm>
 #include <cfloat>
 
@@ -559,10 +560,13 @@ __global__ void __launch_bounds__(kThreads, 1)
 // out[m, n] of 128 weight rows (B's, which take the tensor core's 128 lanes) by MT rows
 // of A, over a part of K per CTA of the cluster. What bounds it is the time to stream the
 // weights, so a CTA's whole part is requested at once as far as shared memory goes; a
-// launch that does next to nothing takes 3.6 us here. Measured, in a graph: 1 x 15360 x 2560
-// nvfp4 5.8 us (3.8 TB/s), 32 x 20480 x 2560 mxfp8 13 us (4.2 TB/s).
+// launch that does next to nothing takes 3.6 us here. Measured, in a graph, weights from
+// memory: 1 x 15360 x 2560 nvfp4 7.5 us (2.9 TB/s; 5.9 where L2 holds them), 32 x 20480 x 2560
+// mxfp8 13 us (4.1 TB/s; 9.3).
 constexpr int kMaxSplits = 8;  // CTAs of a portable cluster
 
+// The 32-row form's ring leaves room for two CTAs on an SM, which share one where there are more
+// tiles than SMs (above 148 x 128 outputs); with fewer, half of the shared memory stays unused.
 template <int FMT, int MT>
 struct SplitCfg {
   using C = StageCfg<FMT, MT, 1>;
